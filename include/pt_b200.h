@@ -416,6 +416,104 @@ PT_B200_API int pt_b200_conv_noalloc(int device, void *stream, const float *x, i
                                      int dil, const float *wp, const float *bias, int epi0,
                                      float a0);
 
+/* ---- Transformer-layer operators (extension) -----------------------------------------------
+ * The layers in front of the decoder (text encoder, flow, duration predictor) are made of linear
+ * layers and layer norms, which the reference's interpreter runs as host ops around
+ * pt_v21_matmul (runtime/v21/src/pt_v21_host.c:3436-3499).  These run them on device buffers the
+ * caller owns, with their gradients.
+ *
+ * Every matrix is row-major with a row stride in elements (at least its column count); rows need
+ * no alignment beyond their element's.  All tensors of a call have one element type.  Sums,
+ * statistics and activations are computed in fp32 and rounded once, to nearest, when stored; an
+ * fp32 call keeps 32-bit accuracy in its products.  Calls are asynchronous on `stream` (NULL: the
+ * default stream) and allocate nothing: workspace comes from the caller, sized by the *_work
+ * function for the same arguments, and is free for reuse once the call's work on the stream is
+ * done.  The status covers argument and launch errors; pt_b200_ops_sync waits for the stream and
+ * reports device errors.  Results do not depend on timing: the same call gives the same bits.
+ * A handle may be used by several threads and streams at once. */
+enum { PT_B200_F32 = 0, PT_B200_BF16 = 1, PT_B200_F16 = 2 };
+/* Activations; 1 and 2 are the conv entry points' epilogue codes. */
+enum {
+  PT_B200_ACT_NONE = 0,
+  PT_B200_ACT_LEAKY = 1, /* p < 0 ? slope * p : p */
+  PT_B200_ACT_RELU = 2,  /* p < 0 ? 0 : p */
+  PT_B200_ACT_GELU = 5,  /* p * Phi(p), Phi the normal distribution function */
+  PT_B200_ACT_SILU = 6   /* p / (1 + exp(-p)) */
+};
+
+typedef struct pt_b200_ops pt_b200_ops;
+/* NULL on failure (no such device, or not a B200). */
+PT_B200_API pt_b200_ops *pt_b200_ops_create(int device);
+PT_B200_API void pt_b200_ops_destroy(pt_b200_ops *h);
+PT_B200_API int pt_b200_ops_sync(pt_b200_ops *h, void *stream);
+
+/* pre = x W^T + bias; y = act(pre) + residual.
+ * x [rows][in], w [out][in], bias [out] or NULL, residual [rows][out] or NULL, y [rows][out];
+ * pre [rows][out] or NULL keeps the value before the activation for the gradient.  y may be the
+ * residual's own buffer (with its stride); no other two tensors may overlap. */
+typedef struct {
+  int32_t dtype, act;
+  int64_t rows, in, out;
+  const void *x, *w, *bias, *residual;
+  void *y, *pre;
+  int64_t ldx, ldw, ldr, ldy, ldp;
+  void *work;
+  int64_t work_bytes;
+  float slope;
+} pt_b200_linear_args;
+PT_B200_API int64_t pt_b200_linear_work(const pt_b200_ops *h, const pt_b200_linear_args *a);
+PT_B200_API int pt_b200_linear(pt_b200_ops *h, void *stream, const pt_b200_linear_args *a);
+
+/* dpre = dy * act'(pre); dx = dpre W; dw = dpre^T x; db = sum over rows of dpre.  Each of dx
+ * [rows][in], dw [out][in], db [out] may be NULL (not computed; then w or x is not needed
+ * either).  pre is needed where act is not NONE.  The residual's gradient is dy itself.  With
+ * bf16 and fp16 tensors dpre is rounded to that type for the two products (db is not affected).
+ * rows = 0 writes zeros to dw and db. */
+typedef struct {
+  int32_t dtype, act;
+  int64_t rows, in, out;
+  const void *dy, *x, *w, *pre;
+  void *dx, *dw, *db;
+  int64_t lddy, ldx, ldw, ldp, lddx, lddw;
+  void *work;
+  int64_t work_bytes;
+  float slope;
+} pt_b200_linear_grad_args;
+PT_B200_API int64_t pt_b200_linear_backward_work(const pt_b200_ops *h, const pt_b200_linear_grad_args *a);
+PT_B200_API int pt_b200_linear_backward(pt_b200_ops *h, void *stream, const pt_b200_linear_grad_args *a);
+
+/* y = (x - mean) * rstd * gamma + beta over each row of x [rows][cols], with rstd = 1 /
+ * sqrt(var + eps) and var the mean squared deviation.  gamma, beta [cols] or NULL (1, 0); mean,
+ * rstd [rows] fp32 or NULL receive the statistics.  y may be x itself (with its stride). */
+typedef struct {
+  int32_t dtype;
+  float eps;
+  int64_t rows, cols;
+  const void *x, *gamma, *beta;
+  void *y;
+  float *mean, *rstd;
+  int64_t ldx, ldy;
+} pt_b200_norm_args;
+PT_B200_API int pt_b200_layer_norm(pt_b200_ops *h, void *stream, const pt_b200_norm_args *a);
+
+/* With g = dy * gamma and xhat = (x - mean) * rstd: dx = rstd * (g - mean(g) - xhat * mean(g *
+ * xhat)); dgamma = sum over rows of dy * xhat; dbeta = sum over rows of dy.  mean and rstd are
+ * the forward pass's.  dx, dgamma and dbeta may each be NULL; dx may be dy itself (with its
+ * stride).  Workspace is needed for dgamma / dbeta only.  rows = 0 writes zeros to dgamma and
+ * dbeta. */
+typedef struct {
+  int32_t dtype, reserved;
+  int64_t rows, cols;
+  const void *dy, *x, *gamma;
+  const float *mean, *rstd;
+  void *dx, *dgamma, *dbeta;
+  int64_t lddy, ldx, lddx;
+  void *work;
+  int64_t work_bytes;
+} pt_b200_norm_grad_args;
+PT_B200_API int64_t pt_b200_layer_norm_backward_work(const pt_b200_ops *h, int64_t rows, int64_t cols);
+PT_B200_API int pt_b200_layer_norm_backward(pt_b200_ops *h, void *stream, const pt_b200_norm_grad_args *a);
+
 /* The tensor core's kind::tf32 rate on `device`, measured live (the conv stack's roofline): one
  * CTA per SM issues `iters` x 4 MMAs of M128 x N256 x K8 from shared-memory operands into TMEM.
  * Returns FLOP per SM clock (averaged over the SMs), the aggregate TFLOP/s over the run, and the

@@ -1,0 +1,113 @@
+// ops.cuh -- shared by the transformer-layer operators (linear.cu, layernorm.cu, ops.cu): element
+// types, activations, the handle, and the launch checks.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/pt_b200.h"
+#include "common.cuh"
+
+struct pt_b200_ops {
+  int device;
+  int sms;
+  uint32_t *gerr;   // device error word: bounded waits that gave up
+};
+
+namespace ptb {
+
+// Makes the handle's device current for one call and puts the caller's back afterwards.
+struct DeviceScope {
+  int prev = -1;
+  bool ok = false;
+  explicit DeviceScope(int device) {
+    int cur = -1;
+    if (cudaGetDevice(&cur) != cudaSuccess) return;
+    if (cur != device) {
+      if (cudaSetDevice(device) != cudaSuccess) return;
+      prev = cur;
+    }
+    ok = true;
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+// ---- element types: every sum, statistic and activation is computed in fp32; a value is rounded
+// to the tensor's type (to nearest even) only when it is stored.
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// V consecutive elements moved as one access (V * sizeof(T) = 16 bytes, or one element).
+template <class T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T v[V];
+};
+
+// Runs fn with a null pointer of the C type that `dtype` names.
+template <class F>
+int with_dtype(int dtype, F &&fn) {
+  switch (dtype) {
+    case PT_B200_F32: return fn(static_cast<float *>(nullptr));
+    case PT_B200_BF16: return fn(static_cast<__nv_bfloat16 *>(nullptr));
+    case PT_B200_F16: return fn(static_cast<__half *>(nullptr));
+  }
+  set_error("pt_b200: unknown element type %d", dtype);
+  return -1;
+}
+inline int dtype_bytes(int dtype) { return dtype == PT_B200_F32 ? 4 : 2; }
+
+// ---- activations.  A NaN passes through each of them; the slope of relu and leaky at 0 is that
+// of the side the comparison puts it on (relu 0, leaky 1).
+constexpr float kSqrtHalf = 0.70710678118654752f;
+constexpr float kInvSqrt2Pi = 0.39894228040143268f;
+
+__device__ __forceinline__ float act_value(float p, int act, float slope) {
+  switch (act) {
+    case PT_B200_ACT_LEAKY: return p < 0.0f ? slope * p : p;
+    case PT_B200_ACT_RELU: return p < 0.0f ? 0.0f : p;
+    case PT_B200_ACT_GELU: return 0.5f * p * (1.0f + erff(p * kSqrtHalf));
+    case PT_B200_ACT_SILU: return p / (1.0f + __expf(-p));
+  }
+  return p;
+}
+
+__device__ __forceinline__ float act_grad(float p, int act, float slope) {
+  switch (act) {
+    case PT_B200_ACT_LEAKY: return p < 0.0f ? slope : 1.0f;
+    case PT_B200_ACT_RELU: return p <= 0.0f ? 0.0f : 1.0f;
+    case PT_B200_ACT_GELU:
+      return 0.5f * (1.0f + erff(p * kSqrtHalf)) + p * kInvSqrt2Pi * __expf(-0.5f * p * p);
+    case PT_B200_ACT_SILU: {
+      const float s = 1.0f / (1.0f + __expf(-p));
+      return s * (1.0f + p * (1.0f - s));
+    }
+  }
+  return 1.0f;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Columns of partial sums [parts][n] -> T out[n], in the partials' order (layernorm.cu).
+template <class T>
+int reduce_columns(const float *part, int parts, int64_t n, T *out, cudaStream_t st);
+
+// ---- argument checks shared by the entry points
+inline bool rows_ok(const void *p, int64_t rows, int64_t cols, int64_t ld, int bytes) {
+  return rows == 0 || (p && ld >= cols && (reinterpret_cast<uintptr_t>(p) % bytes) == 0);
+}
+
+}  // namespace ptb

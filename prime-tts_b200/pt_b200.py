@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import subprocess
 from dataclasses import dataclass, field
 
@@ -160,6 +161,16 @@ _SIGS = {
     "pt_b200_decoder_create_from_ptk": ([C.c_int, C.c_char_p], C.c_void_p),
     "pt_b200_mma_rate": ([C.c_int, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_double),
                           C.POINTER(C.c_double)], C.c_int),
+    "pt_b200_ops_create": ([C.c_int], C.c_void_p),
+    "pt_b200_ops_destroy": ([C.c_void_p], None),
+    "pt_b200_ops_sync": ([C.c_void_p, C.c_void_p], C.c_int),
+    "pt_b200_linear_work": ([C.c_void_p, C.c_char_p], _i64),
+    "pt_b200_linear": ([C.c_void_p, C.c_void_p, C.c_char_p], C.c_int),
+    "pt_b200_linear_backward_work": ([C.c_void_p, C.c_char_p], _i64),
+    "pt_b200_linear_backward": ([C.c_void_p, C.c_void_p, C.c_char_p], C.c_int),
+    "pt_b200_layer_norm": ([C.c_void_p, C.c_void_p, C.c_char_p], C.c_int),
+    "pt_b200_layer_norm_backward_work": ([C.c_void_p, _i64, _i64], _i64),
+    "pt_b200_layer_norm_backward": ([C.c_void_p, C.c_void_p, C.c_char_p], C.c_int),
     "pt_b200_last_error": ([], C.c_char_p),
     "pt_b200_kernel_launches": ([C.c_int], C.c_long),
 }
@@ -770,3 +781,228 @@ class Decoder:
             _check(k, "pt_b200_decoder_launch_times")
         return [(self.LAUNCH_KINDS[kd[i] & 255], kd[i] >> 8, ms[i], fl[i], by[i])
                 for i in range(k)]
+
+
+# --------------------------------------------------------------------------------------------
+class Operators:
+    """The transformer-layer operators on torch CUDA tensors (pt_b200_ops_*): the linear layer with
+    its fused epilogue and the layer norm, forward and backward.
+
+    Tensors are float32, bfloat16 or float16, all of a call of one type and on this device; a matrix
+    is [..., columns] with contiguous columns and one stride for its rows (a column slice of a wider
+    tensor is fine).  Calls run on torch's current stream and return without waiting; outputs and
+    workspaces come from torch's allocator.  Nothing is recorded for autograd.  A bad argument
+    raises PtB200Error before anything is launched; sync() waits and reports device errors."""
+
+    ACTS = {"none": 0, "leaky": 1, "relu": 2, "gelu": 5, "silu": 6}
+    # the argument structs of include/pt_b200.h, packed field by field
+    _LINEAR = struct.Struct("=2i3q4Q2Q5qQqf4x")
+    _LINEAR_GRAD = struct.Struct("=2i3q4Q3Q6qQqf4x")
+    _NORM = struct.Struct("=if2q3QQ2Q2q")
+    _NORM_GRAD = struct.Struct("=2i2q3Q2Q3Q3qQq")
+
+    def __init__(self, device: int = 0):
+        import torch
+        self._torch = torch
+        self._lib = lib()
+        self.h = None
+        h = self._lib.pt_b200_ops_create(device)
+        if not h:
+            _check(-1, "pt_b200_ops_create")
+        self.h = h
+        self.device = device
+        self._types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+    def close(self) -> None:
+        if self.h:
+            self._lib.pt_b200_ops_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def sync(self) -> None:
+        """Wait for torch's current stream and report device errors."""
+        _check(self._lib.pt_b200_ops_sync(self.h, self._stream()), "pt_b200_ops_sync")
+
+    def _stream(self) -> int:
+        return self._torch.cuda.current_stream(self.device).cuda_stream
+
+    def _type(self, t, what: str) -> int:
+        """The element type of a call's first tensor."""
+        code = self._types.get(t.dtype)
+        if code is None or t.get_device() != self.device:
+            raise PtB200Error(f"{what}: needs a float32, bfloat16 or float16 tensor on cuda:"
+                              f"{self.device}, got {t.dtype} on {t.device}")
+        return code
+
+    def _rows(self, t, name: str, dtype, rows: int, cols: int):
+        """(address, row stride) of a [..., cols] tensor seen as [rows][cols]."""
+        shape = t.shape
+        if t.dtype != dtype or t.get_device() != self.device or len(shape) < 1 or shape[-1] != cols \
+                or t.numel() != rows * cols:
+            raise PtB200Error(f"{name}: needs {rows} rows of {cols} {dtype} on cuda:{self.device}, got "
+                              f"{tuple(shape)} {t.dtype} on {t.device}")
+        if len(shape) != 2:
+            try:
+                t = t.view(rows, cols)
+            except RuntimeError:
+                raise PtB200Error(f"{name}: its leading dimensions have no common row stride") from None
+        ld, step = t.stride()
+        if step != 1 and cols > 1 and rows > 0:
+            raise PtB200Error(f"{name}: its columns are not contiguous (stride {step})")
+        if ld < cols:
+            if rows > 1:
+                raise PtB200Error(f"{name}: its rows overlap (stride {ld} for {cols} columns)")
+            ld = cols
+        return t.data_ptr(), ld
+
+    def _vector(self, t, name: str, dtype, n: int) -> int:
+        """The address of a contiguous [n] tensor, 0 for None."""
+        if t is None:
+            return 0
+        if t.dtype != dtype or t.get_device() != self.device or t.dim() != 1 or t.shape[0] != n \
+                or (n > 1 and t.stride(0) != 1):
+            raise PtB200Error(f"{name}: needs {n} contiguous {dtype} on cuda:{self.device}, got "
+                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        return t.data_ptr()
+
+    def _flat(self, t, name: str, dtype, n: int) -> int:
+        """The address of a contiguous tensor of n elements, whatever its shape."""
+        return self._vector(t if t.dim() == 1 or not t.is_contiguous() else t.view(-1), name, dtype, n)
+
+    def _act(self, act: str) -> int:
+        code = self.ACTS.get(act)
+        if code is None:
+            raise PtB200Error(f"act is one of {', '.join(self.ACTS)}, got {act!r}")
+        return code
+
+    def _workspace(self, n: int):
+        return self._torch.empty(n, dtype=self._torch.uint8, device=self.device) if n else None
+
+    def linear(self, x, w, bias=None, residual=None, act: str = "none", slope: float = 0.1,
+               save_pre: bool = False):
+        """act(x W^T + bias) + residual for x [..., in], w [out][in]; [..., out].  With save_pre
+        also the value before the activation, as linear_backward wants it: (y, pre)."""
+        code, dt, empty = self._type(x, "x"), x.dtype, self._torch.empty
+        if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+            raise PtB200Error(f"linear: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit")
+        n_out, n_in = w.shape
+        if n_in == 0 or n_out == 0:
+            raise PtB200Error(f"linear: w {tuple(w.shape)} is empty")
+        rows = x.numel() // n_in
+        xp, ldx = self._rows(x, "x", dt, rows, n_in)
+        wp, ldw = self._rows(w, "w", dt, n_out, n_in)
+        bp = self._vector(bias, "bias", dt, n_out)
+        rp, ldr = self._rows(residual, "residual", dt, rows, n_out) if residual is not None else (0, 0)
+        shape = x.shape[:-1] + (n_out,)
+        y = empty(shape, dtype=dt, device=x.device)
+        pre = empty(shape, dtype=dt, device=x.device) if save_pre else None
+
+        def pack(work, nbytes):
+            return self._LINEAR.pack(code, self._act(act), rows, n_in, n_out, xp, wp, bp, rp,
+                                     y.data_ptr(), pre.data_ptr() if save_pre else 0, ldx, ldw, ldr,
+                                     n_out, n_out, work, nbytes, slope)
+
+        args = pack(0, 0)
+        need = self._lib.pt_b200_linear_work(self.h, args)
+        if need:
+            work = self._workspace(need)
+            args = pack(work.data_ptr(), need)
+        if self._lib.pt_b200_linear(self.h, self._stream(), args):
+            _check(-1, "pt_b200_linear")
+        return (y, pre) if save_pre else y
+
+    def linear_backward(self, dy, x, w, pre=None, act: str = "none", slope: float = 0.1,
+                        need_dx: bool = True, need_dw: bool = True, need_db: bool = True):
+        """(dx, dw, db) of linear for dy [..., out]; None in the place of one not asked for.  pre is
+        what linear(save_pre=True) kept, needed where there is an activation."""
+        code, dt, empty = self._type(dy, "dy"), dy.dtype, self._torch.empty
+        if w.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != w.shape[0]:
+            raise PtB200Error(f"linear_backward: dy {tuple(dy.shape)} and w {tuple(w.shape)} do not fit")
+        n_out, n_in = w.shape
+        if n_in == 0 or n_out == 0:
+            raise PtB200Error(f"linear_backward: w {tuple(w.shape)} is empty")
+        if not (need_dx or need_dw or need_db):
+            raise PtB200Error("linear_backward: nothing to compute")
+        rows = dy.numel() // n_out
+        a = self._act(act)
+        if a and pre is None:
+            raise PtB200Error(f"linear_backward: act {act!r} needs pre")
+        gp, lddy = self._rows(dy, "dy", dt, rows, n_out)
+        xp, ldx = self._rows(x, "x", dt, rows, n_in)
+        wp, ldw = self._rows(w, "w", dt, n_out, n_in)
+        pp, ldp = self._rows(pre, "pre", dt, rows, n_out) if a else (0, 0)
+        dev = dy.device
+        dx = empty(dy.shape[:-1] + (n_in,), dtype=dt, device=dev) if need_dx else None
+        dw = empty((n_out, n_in), dtype=dt, device=dev) if need_dw else None
+        db = empty((n_out,), dtype=dt, device=dev) if need_db else None
+
+        def pack(work, nbytes):
+            return self._LINEAR_GRAD.pack(code, a, rows, n_in, n_out, gp, xp, wp, pp,
+                                          dx.data_ptr() if need_dx else 0,
+                                          dw.data_ptr() if need_dw else 0,
+                                          db.data_ptr() if need_db else 0, lddy, ldx, ldw, ldp,
+                                          n_in, n_in, work, nbytes, slope)
+
+        args = pack(0, 0)
+        need = self._lib.pt_b200_linear_backward_work(self.h, args)
+        if need:
+            work = self._workspace(need)
+            args = pack(work.data_ptr(), need)
+        if self._lib.pt_b200_linear_backward(self.h, self._stream(), args):
+            _check(-1, "pt_b200_linear_backward")
+        return dx, dw, db
+
+    def layer_norm(self, x, gamma=None, beta=None, eps: float = 1e-5):
+        """Layer norm over the last dimension: (y, mean, rstd), the statistics in float32."""
+        code, dt, torch = self._type(x, "x"), x.dtype, self._torch
+        cols = x.shape[-1] if x.dim() else 0
+        if cols == 0:
+            raise PtB200Error(f"layer_norm: x {tuple(x.shape)} has no columns")
+        rows = x.numel() // cols
+        xp, ldx = self._rows(x, "x", dt, rows, cols)
+        gp, bp = self._vector(gamma, "gamma", dt, cols), self._vector(beta, "beta", dt, cols)
+        y = torch.empty(x.shape, dtype=dt, device=x.device)
+        stat = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+        mean, rstd = stat[0], stat[1]
+        sp = stat.data_ptr()
+        args = self._NORM.pack(code, eps, rows, cols, xp, gp, bp, y.data_ptr(), sp, sp + 4 * rows, ldx,
+                               cols)
+        if self._lib.pt_b200_layer_norm(self.h, self._stream(), args):
+            _check(-1, "pt_b200_layer_norm")
+        return y, mean, rstd
+
+    def layer_norm_backward(self, dy, x, gamma, mean, rstd, need_dx: bool = True,
+                            need_dgamma: bool = True, need_dbeta: bool = True):
+        """(dx, dgamma, dbeta) of layer_norm; None in the place of one not asked for."""
+        code, dt, empty = self._type(dy, "dy"), dy.dtype, self._torch.empty
+        cols = dy.shape[-1] if dy.dim() else 0
+        if cols == 0:
+            raise PtB200Error(f"layer_norm_backward: dy {tuple(dy.shape)} has no columns")
+        if not (need_dx or need_dgamma or need_dbeta):
+            raise PtB200Error("layer_norm_backward: nothing to compute")
+        rows, dev = dy.numel() // cols, dy.device
+        yp, lddy = self._rows(dy, "dy", dt, rows, cols)
+        xp, ldx = self._rows(x, "x", dt, rows, cols)
+        gp = self._vector(gamma, "gamma", dt, cols)
+        f32 = self._torch.float32
+        mp, rp = self._flat(mean, "mean", f32, rows), self._flat(rstd, "rstd", f32, rows)
+        dx = empty(dy.shape, dtype=dt, device=dev) if need_dx else None
+        dgamma = empty((cols,), dtype=dt, device=dev) if need_dgamma else None
+        dbeta = empty((cols,), dtype=dt, device=dev) if need_dbeta else None
+        need = 0
+        if need_dgamma or need_dbeta:
+            need = self._lib.pt_b200_layer_norm_backward_work(self.h, rows, cols)
+        work = self._workspace(need)
+        args = self._NORM_GRAD.pack(code, 0, rows, cols, yp, xp, gp, mp, rp,
+                                    dx.data_ptr() if need_dx else 0,
+                                    dgamma.data_ptr() if need_dgamma else 0,
+                                    dbeta.data_ptr() if need_dbeta else 0, lddy, ldx, cols,
+                                    work.data_ptr() if need else 0, need)
+        if self._lib.pt_b200_layer_norm_backward(self.h, self._stream(), args):
+            _check(-1, "pt_b200_layer_norm_backward")
+        return dx, dgamma, dbeta
