@@ -425,8 +425,9 @@ PT_B200_API int pt_b200_conv_noalloc(int device, void *stream, const float *x, i
  * Every matrix is row-major with a row stride in elements (at least its column count); rows need
  * no alignment beyond their element's.  All tensors of a call have one element type.  Sums,
  * statistics and activations are computed in fp32 and rounded once, to nearest, when stored; an
- * fp32 call keeps 32-bit accuracy in its products.  Calls are asynchronous on `stream` (NULL: the
- * default stream) and allocate nothing: workspace comes from the caller, sized by the *_work
+ * fp32 call keeps 32-bit accuracy in its products (an infinite fp32 input makes the outputs that
+ * depend on it NaN or infinite).  Calls are asynchronous on `stream` (NULL: the default stream)
+ * and allocate nothing: workspace (256-byte aligned) comes from the caller, sized by the *_work
  * function for the same arguments, and is free for reuse once the call's work on the stream is
  * done.  The status covers argument and launch errors; pt_b200_ops_sync waits for the stream and
  * reports device errors.  Results do not depend on timing: the same call gives the same bits.

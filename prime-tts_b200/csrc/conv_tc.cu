@@ -49,6 +49,8 @@ static int encoder(PFN_cuTensorMapEncodeTiled_v12000 *fn) {
   return 0;
 }
 
+int tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000 *fn) { return encoder(fn); }
+
 int make_map_act(CUtensorMap *m, const float *base, int cin32, int64_t rows, int batch,
                  int box_rows) {
   PFN_cuTensorMapEncodeTiled_v12000 enc;

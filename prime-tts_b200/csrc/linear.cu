@@ -3,8 +3,8 @@
 //   pre = x W^T + b;  y = act(pre) + r
 //   dpre = dy * act'(pre);  dx = dpre W;  dW = dpre^T x;  db = sum over rows of dpre
 //
-// All three products are D[m][n] = sum_k A(m, k) B(n, k) over operands read along either index.
-#include "linear.cuh"
+// The three products run on the tensor cores (linear_tc.cu).
+#include "linear_tc.cuh"
 
 using namespace ptb;
 
@@ -12,71 +12,12 @@ namespace {
 
 constexpr int kBlock = 256;
 
-// ---- fp32 FMA product for every type, stride and size: 64 x 64 outputs per block, 4 x 4 per
-// thread, operands staged 16 deep in shared memory as fp32.
-constexpr int kTile = 64, kDepth = 16;
-
-template <class T>
-__global__ void __launch_bounds__(kBlock) product_kernel(const LinearProduct p) {
-  __shared__ float sa[kDepth][kTile + 4], sb[kDepth][kTile + 4];
-  const int64_t tn = (p.n + kTile - 1) / kTile;
-  const int64_t m0 = blockIdx.x / tn * kTile, n0 = blockIdx.x % tn * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const T *a = static_cast<const T *>(p.a), *b = static_cast<const T *>(p.b);
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
-#pragma unroll
-    for (int i = 0; i < kTile * kDepth / kBlock; ++i) {
-      const int e = i * kBlock + threadIdx.x;
-      // consecutive threads follow the index that is contiguous in memory
-      const int ka = p.a_k == 1 ? e % kDepth : e / kTile, ra = p.a_k == 1 ? e / kDepth : e % kTile;
-      const int kb = p.b_k == 1 ? e % kDepth : e / kTile, rb = p.b_k == 1 ? e / kDepth : e % kTile;
-      sa[ka][ra] = m0 + ra < p.m && k0 + ka < p.k
-                       ? to_f32(a[(m0 + ra) * p.a_m + (k0 + ka) * p.a_k]) : 0.0f;
-      sb[kb][rb] = n0 + rb < p.n && k0 + kb < p.k
-                       ? to_f32(b[(n0 + rb) * p.b_n + (k0 + kb) * p.b_k]) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kDepth; ++k) {
-      float va[4], vb[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        va[i] = sa[k][ty * 4 + i];
-        vb[i] = sb[k][tx + 16 * i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(va[i], vb[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (m0 + ty * 4 + i < p.m && n0 + tx + 16 * j < p.n)
-        linear_store<T>(p.e, m0 + ty * 4 + i, n0 + tx + 16 * j, acc[i][j]);
-}
-
-template <class T>
-int launch_product(const LinearProduct &p, cudaStream_t st) {
-  const int64_t tiles = ((p.m + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile);
-  PTB_REQUIRE(tiles < (int64_t(1) << 31), "pt_b200: product of %lld x %lld is too large", (long long)p.m,
-              (long long)p.n);
-  product_kernel<T><<<static_cast<unsigned>(tiles), kBlock, 0, st>>>(p);
-  PTB_CUDA(cudaGetLastError());
-  count_launch();
-  return 0;
-}
-
 // ---- dpre = dy * act'(pre), and its column sums as one row of partials per blockIdx.y
 struct GradArgs {
   const void *dy, *pre;
-  void *g;               // dpre, or null (no activation: dpre is dy itself)
+  void *g;               // dpre as the products read it, or null
   float *part;           // [gridDim.y][n], or null
-  int64_t rows, n, lddy, ldp, ldg;
+  int64_t rows, n, lddy, ldp, ldg, plane;
   int act;
   float slope;
 };
@@ -91,9 +32,21 @@ __global__ void __launch_bounds__(kBlock) act_grad_kernel(const GradArgs a) {
     for (int64_t r = static_cast<int64_t>(blockIdx.y) * 8 + lane; r < a.rows;
          r += static_cast<int64_t>(gridDim.y) * 8) {
       float d = to_f32(static_cast<const T *>(a.dy)[r * a.lddy + c]);
-      if (a.act) d *= act_grad(to_f32(static_cast<const T *>(a.pre)[r * a.ldp + c]), a.act, a.slope);
+      // (an explicit product: the sum must not depend on whether d is also stored)
+      if (a.act)
+        d = __fmul_rn(d, act_grad(to_f32(static_cast<const T *>(a.pre)[r * a.ldp + c]), a.act, a.slope));
       // rounded to the operands' type for the two products; the sums take the fp32 value
-      if (a.g) static_cast<T *>(a.g)[r * a.ldg + c] = from_f32<T>(d);
+      if (a.g) {
+        if constexpr (sizeof(T) == 4) {
+          __nv_bfloat16 o[3];
+          split3(d, o);
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            static_cast<__nv_bfloat16 *>(a.g)[p * a.plane + r * a.ldg + c] = o[p];
+        } else {
+          static_cast<T *>(a.g)[r * a.ldg + c] = from_f32<T>(d);
+        }
+      }
       sum += d;
     }
   if (!a.part) return;
@@ -111,7 +64,26 @@ int grad_parts(int64_t rows) {
   return static_cast<int>(n < 64 ? n : 64);
 }
 
-int64_t up256(int64_t b) { return (b + 255) / 256 * 256; }
+// An operand: the tensor itself where the tensor cores can read it, else its planes at *work.
+struct Operand {
+  bool direct;
+  int64_t bytes;
+};
+Operand operand(int dtype, const void *p, int64_t rows, int64_t cols, int64_t ld) {
+  const bool direct = tc_direct(dtype, p, rows, ld);
+  return Operand{direct, direct ? 0 : tc_plane_bytes(dtype, rows, cols)};
+}
+int prepare(const pt_b200_ops *h, int dtype, const void *p, int64_t rows, int64_t cols, int64_t ld, char **work,
+            TcOperand *out, cudaStream_t st) {
+  const Operand o = operand(dtype, p, rows, cols, ld);
+  if (o.direct) {
+    *out = tc_tensor(p, rows, cols, ld);
+    return 0;
+  }
+  *out = tc_planes(*work, rows, cols);
+  *work += o.bytes;
+  return tc_pack(h, dtype, p, ld, *out, st);
+}
 
 bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
   return rows >= 0 && n_in > 0 && n_out > 0 && rows < (int64_t(1) << 31) && n_in < (int64_t(1) << 30) &&
@@ -121,9 +93,9 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
 }  // namespace
 
 extern "C" int64_t pt_b200_linear_work(const pt_b200_ops *h, const pt_b200_linear_args *p) {
-  (void)h;
-  (void)p;
-  return 0;
+  if (!h || !p || !sizes_ok(p->rows, p->in, p->out) || p->rows == 0) return 0;
+  return operand(p->dtype, p->x, p->rows, p->in, p->ldx).bytes +
+         operand(p->dtype, p->w, p->out, p->in, p->ldw).bytes;
 }
 
 extern "C" int pt_b200_linear(pt_b200_ops *h, void *stream, const pt_b200_linear_args *p) {
@@ -145,18 +117,34 @@ extern "C" int pt_b200_linear(pt_b200_ops *h, void *stream, const pt_b200_linear
   DeviceScope on(h->device);
   PTB_REQUIRE(on.ok, "pt_b200_linear: device %d cannot be used", h->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  LinearProduct q{p->x, p->w, p->ldx, 1, p->ldw, 1, p->rows, p->out, p->in,
-                  {p->bias, p->residual, p->y, p->pre, p->ldr, p->ldy, p->ldp, p->act, p->slope}};
-  return with_dtype(p->dtype, [&](auto *z) -> int {
-    return launch_product<std::remove_pointer_t<decltype(z)>>(q, st);
-  });
+  const int64_t need = pt_b200_linear_work(h, p);
+  PTB_REQUIRE(need == 0 || (p->work && p->work_bytes >= need && reinterpret_cast<uintptr_t>(p->work) % 256 == 0),
+              "pt_b200_linear: %lld bytes of 256-byte aligned workspace are needed, %lld given", (long long)need,
+              (long long)p->work_bytes);
+  char *work = static_cast<char *>(p->work);
+  TcProduct q{};
+  if (prepare(h, p->dtype, p->w, p->out, p->in, p->ldw, &work, &q.a, st) ||
+      prepare(h, p->dtype, p->x, p->rows, p->in, p->ldx, &work, &q.b, st))
+    return -1;
+  q.rows = p->rows;
+  q.chans = p->out;
+  q.k = p->in;
+  q.e = LinearEpi{p->bias, p->residual, p->y, p->pre, p->ldr, p->ldy, p->ldp, p->act, p->slope};
+  return tc_product(h, p->dtype, q, st);
+}
+
+// The gradient's operand dpre is dy itself where nothing has to be computed or copied for it.
+static bool grad_direct(const pt_b200_linear_grad_args *p) {
+  return p->act == PT_B200_ACT_NONE && tc_direct(p->dtype, p->dy, p->rows, p->lddy);
 }
 
 extern "C" int64_t pt_b200_linear_backward_work(const pt_b200_ops *h, const pt_b200_linear_grad_args *p) {
   if (!h || !p || !sizes_ok(p->rows, p->in, p->out) || p->rows == 0) return 0;
   int64_t need = 0;
-  if (p->act != PT_B200_ACT_NONE) need += up256(p->rows * p->out * dtype_bytes(p->dtype));
-  if (p->db) need += up256(static_cast<int64_t>(grad_parts(p->rows)) * p->out * 4);
+  if ((p->dx || p->dw) && !grad_direct(p)) need += tc_plane_bytes(p->dtype, p->rows, p->out);
+  if (p->dx) need += operand(p->dtype, p->w, p->out, p->in, p->ldw).bytes;
+  if (p->dw) need += operand(p->dtype, p->x, p->rows, p->in, p->ldx).bytes;
+  if (p->db) need += static_cast<int64_t>(grad_parts(p->rows)) * p->out * 4;
   return need;
 }
 
@@ -188,21 +176,25 @@ extern "C" int pt_b200_linear_backward(pt_b200_ops *h, void *stream, const pt_b2
     return 0;
   }
   const int64_t need = pt_b200_linear_backward_work(h, p);
-  PTB_REQUIRE(need == 0 || (p->work && p->work_bytes >= need && reinterpret_cast<uintptr_t>(p->work) % 16 == 0),
-              "pt_b200_linear_backward: %lld bytes of 16-byte aligned workspace are needed, %lld given",
+  PTB_REQUIRE(need == 0 || (p->work && p->work_bytes >= need && reinterpret_cast<uintptr_t>(p->work) % 256 == 0),
+              "pt_b200_linear_backward: %lld bytes of 256-byte aligned workspace are needed, %lld given",
               (long long)need, (long long)p->work_bytes);
   return with_dtype(p->dtype, [&](auto *z) -> int {
     using T = std::remove_pointer_t<decltype(z)>;
     char *work = static_cast<char *>(p->work);
-    const void *g = p->dy;
-    int64_t ldg = p->lddy;
-    GradArgs ga{p->dy, p->pre, nullptr, nullptr, p->rows, p->out, p->lddy, p->ldp, p->out, p->act, p->slope};
-    if (acts) {
+    TcOperand g = tc_tensor(p->dy, p->rows, p->out, p->lddy);
+    GradArgs ga{p->dy, p->pre, nullptr, nullptr, p->rows, p->out, p->lddy, p->ldp, 0, 0, p->act, p->slope};
+    if ((p->dx || p->dw) && !grad_direct(p)) {
+      g = tc_planes(work, p->rows, p->out);
       ga.g = work;
-      g = work;
-      ldg = p->out;
-      work += up256(p->rows * p->out * eb);
+      ga.ldg = g.ld;
+      ga.plane = g.plane;
+      work += tc_plane_bytes(p->dtype, p->rows, p->out);
     }
+    TcProduct dx{}, dw{};
+    if ((p->dx && prepare(h, p->dtype, p->w, p->out, p->in, p->ldw, &work, &dx.a, st)) ||
+        (p->dw && prepare(h, p->dtype, p->x, p->rows, p->in, p->ldx, &work, &dw.a, st)))
+      return -1;
     if (p->db) ga.part = reinterpret_cast<float *>(work);
     if (ga.g || ga.part) {
       const int parts = grad_parts(p->rows);
@@ -211,18 +203,25 @@ extern "C" int pt_b200_linear_backward(pt_b200_ops *h, void *stream, const pt_b2
       count_launch();
       if (p->db && reduce_columns<T>(ga.part, parts, p->out, static_cast<T *>(p->db), st)) return -1;
     }
-    LinearEpi plain{};
     if (p->dx) {
-      LinearProduct q{g, p->w, ldg, 1, 1, p->ldw, p->rows, p->in, p->out, plain};
-      q.e.y = p->dx;
-      q.e.ldy = p->lddx;
-      if (launch_product<T>(q, st)) return -1;
+      dx.b = g;
+      dx.a_mn = true;
+      dx.rows = p->rows;
+      dx.chans = p->in;
+      dx.k = p->out;
+      dx.e.y = p->dx;
+      dx.e.ldy = p->lddx;
+      if (tc_product(h, p->dtype, dx, st)) return -1;
     }
     if (p->dw) {
-      LinearProduct q{g, p->x, 1, ldg, 1, p->ldx, p->out, p->in, p->rows, plain};
-      q.e.y = p->dw;
-      q.e.ldy = p->lddw;
-      if (launch_product<T>(q, st)) return -1;
+      dw.b = g;
+      dw.a_mn = dw.b_mn = true;
+      dw.rows = p->out;
+      dw.chans = p->in;
+      dw.k = p->rows;
+      dw.e.y = p->dw;
+      dw.e.ldy = p->lddw;
+      if (tc_product(h, p->dtype, dw, st)) return -1;
     }
     return 0;
   });

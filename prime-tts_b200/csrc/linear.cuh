@@ -16,14 +16,6 @@ struct LinearEpi {
   float slope;
 };
 
-// D[m][n] = sum_k A(m, k) B(n, k), each operand with a stride per index (in elements).
-struct LinearProduct {
-  const void *a, *b;
-  int64_t a_m, a_k, b_n, b_k;
-  int64_t m, n, k;
-  LinearEpi e;
-};
-
 template <class T>
 __device__ __forceinline__ void linear_store(const LinearEpi &e, int64_t m, int64_t n, float v) {
   if (e.bias) v += to_f32(static_cast<const T *>(e.bias)[n]);
