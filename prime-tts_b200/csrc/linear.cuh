@@ -16,11 +16,17 @@ struct LinearEpi {
   float slope;
 };
 
+struct ActOnOne {
+  float &v;
+  float slope;
+  template <int ACT>
+  __device__ __forceinline__ void operator()() const { v = act_value<ACT>(v, slope); }
+};
 template <class T>
 __device__ __forceinline__ void linear_store(const LinearEpi &e, int64_t m, int64_t n, float v) {
   if (e.bias) v += to_f32(static_cast<const T *>(e.bias)[n]);
   if (e.pre) static_cast<T *>(e.pre)[m * e.ldp + n] = from_f32<T>(v);
-  v = act_value(v, e.act, e.slope);
+  with_act(e.act, ActOnOne{v, e.slope});
   if (e.residual) v += to_f32(static_cast<const T *>(e.residual)[m * e.ldr + n]);
   static_cast<T *>(e.y)[m * e.ldy + n] = from_f32<T>(v);
 }

@@ -22,9 +22,13 @@
 // k starts a new accumulator and the epilogue warps add the chunks in registers, rounding to
 // nearest.
 //
-// One CTA per SM walks its tiles: a TMA producer warp, an MMA warp, eight epilogue warps.  Two
-// accumulators in TMEM let the epilogue of one tile run beside the next tile's MMAs.  When there
-// are fewer tiles than SMs, a cluster of CTAs shares a tile's k range: each leaves its part in its
+// One CTA per SM walks its tiles: a TMA producer warp, an MMA warp, sixteen epilogue warps.  Two
+// accumulators in TMEM let the epilogue of one tile run beside the next tile's MMAs.
+//
+// Large products run on CTA pairs (G = 2): one MMA of 256 channels over both SMs, each holding its
+// 128 channels of A and half of the tile's rows of B, so that an SM reads and fetches half as much
+// of B for the same arithmetic.  Products of few tiles run on single CTAs, and when there are
+// fewer tiles than SMs a cluster of them shares a tile's k range: each leaves its part in its
 // shared memory and adds a slice of the columns from all of them through distributed shared
 // memory, in the order of the parts.
 #include <cooperative_groups.h>
@@ -43,12 +47,35 @@ int tensor_map_encoder(PFN_cuTensorMapEncodeTiled_v12000 *fn);   // conv_tc.cu
 
 namespace {
 
-constexpr int kEpiWarps = 8;
-constexpr int kTcThreads = (4 + kEpiWarps) * 32;   // warp 0 TMA, warp 1 MMA, 2-3 idle, 4-11 epilogue
+constexpr int kEpiWarps = 16;   // four to a quarter of the lanes: two left an epilogue of gelu and two stores latency-bound
+constexpr int kFirstEpi = 3;
+constexpr int kTcThreads = (kFirstEpi + kEpiWarps) * 32;   // warps 0 and 2 copy A and B, warp 1 MMA, the rest epilogue
 constexpr int kM = 128;
+constexpr int kMaxBn1 = 256, kMaxBn3 = 192;   // rows per tile; three planes' sums are in registers
+constexpr int KB = 64;   // elements of k per stage: a 128-byte row
 constexpr int kMaxStages = 10;
+constexpr int kMaxSplit = 8;
 constexpr int kSmemBudget = 217 * 1024;
-constexpr int kSmemBytes = kSmemBudget + 1024 + 512;
+constexpr int kSumLanes = 8;
+constexpr int kSumBytes = kSumLanes * 33 * 4;
+constexpr int kSmemBytes = kSmemBudget + 1024 + 512 + kSumBytes;
+
+// t / d for 0 <= t < 2^31 as a multiplication: mul = ceil(2^(31 + s) / d) with 2^s >= d is off by
+// less than 2^s / 2^31 of a quotient step, which t cannot make up.
+struct Divide {
+  uint32_t mul;
+  int shift;
+  explicit Divide(uint32_t d = 1) {
+    int s = 0;
+    while ((1u << s) < d) ++s;
+    mul = static_cast<uint32_t>(((uint64_t(1) << (31 + s)) + d - 1) / d);
+    shift = 31 + s;
+  }
+  __device__ __forceinline__ int of(int t) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(t)) * mul) >> shift);
+  }
+};
+constexpr int kBand = 16;
 
 struct TcArgs {
   LinearEpi e;
@@ -59,47 +86,133 @@ struct TcArgs {
   int bn;                   // rows per tile
   int stages;
   int tiles_m, tiles_n;     // channel tiles, row tiles
+  Divide by_band;           // by the tiles of a band
+  Divide by_last;           // by the channel tiles of the last band, where it is not a whole one
   uint32_t idesc;
   bool a_mn, b_mn;
+  bool beside;              // needs nothing of the kernel launched right before it
+  ColumnSums sums;          // done beside the first tile, or parts = 0
 };
 
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
+// ---- the same steps for one CTA (G = 1) and for a pair (G = 2, issued by its rank 0)
+// Descriptors come as their low words (the address moves, 16 bytes a step) and the constant high
+// word; FIRST starts the accumulator where `keep` is 0, any other MMA adds to it.
+template <int G, bool FIRST>
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                        uint32_t keep) {
+#define PTB_MMA(group, pred)                                                                              \
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"                                               \
+               "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t" pred                                   \
+               "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),        \
+               "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(keep)                                       \
+               : "memory")
+  if constexpr (G == 1 && FIRST) PTB_MMA("1", "setp.ne.b32 p, %5, 0;\n\t");
+  if constexpr (G == 1 && !FIRST) PTB_MMA("1", "setp.ne.b32 p, 1, 0;\n\t");
+  if constexpr (G == 2 && FIRST) PTB_MMA("2", "setp.ne.b32 p, %5, 0;\n\t");
+  if constexpr (G == 2 && !FIRST) PTB_MMA("2", "setp.ne.b32 p, 1, 0;\n\t");
+#undef PTB_MMA
+}
+// Arrives on the barrier at this offset, of both CTAs of a pair, once the MMAs so far are done.
+template <int G>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (G == 1)
+    mma_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+template <int G>
+__device__ __forceinline__ void alloc(uint32_t slot, uint32_t cols) {
+  if constexpr (G == 1) {
+    tmem_alloc(slot, cols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int G>
+__device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t cols) {
+  if constexpr (G == 1)
+    tmem_dealloc(taddr, cols);
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+// A tile into this CTA's shared memory; `bar` may be the other CTA's of the pair.
+template <int G>
+__device__ __forceinline__ void load(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1, int c2) {
+  if constexpr (G == 1)
+    tma_load_3d(dst, map, bar, c0, c1, c2);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+// True in one lane of the warp.  The roles below run with all lanes, so that their loop state is
+// the same in every lane and stays in uniform registers, and only the copies and MMAs themselves
+// are issued by one: with the whole loop inside one lane's branch, an MMA took 140 clocks to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+// The same value in every lane, and known to be.
+template <class V>
+__device__ __forceinline__ V uniform(V v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ uint32_t in_rank0(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+// An accumulator is free again.  Only TMEM loads, already waited for, come before it: no memory has
+// to be released, and a cluster-wide release took 1100 to 3800 clocks of every chunk.
+template <int G>
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  if constexpr (G == 1)
+    mbar_arrive(bar);
+  else
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Shared-memory descriptors.  K-major: rows of KB elements (128 or 64 bytes, swizzled by as much),
-// 8-row atoms one after another.  MN-major: blocks of 64 elements (128 bytes, swizzled) x KB k
-// rows; `lead` bytes from one block of 64 to the next, 8 k rows to an atom of 1024 bytes.
-__device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lead, uint32_t atom, uint32_t swizzle) {
-  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | static_cast<uint64_t>((lead >> 4) & 0x3FFFu) << 16 |
-         static_cast<uint64_t>((atom >> 4) & 0x3FFFu) << 32 | static_cast<uint64_t>(1u) << 46 |
-         static_cast<uint64_t>(swizzle) << 61;
+// Shared-memory descriptors.  K-major: rows of KB = 64 elements (128 bytes, swizzled by as much),
+// atoms of 8 rows one after another.  MN-major: blocks of 64 elements (128 bytes, swizzled) x KB
+// rows of k; `lead` bytes from one block of 64 to the next, 8 rows of k to an atom.
+__device__ __forceinline__ uint32_t sdesc_lo(uint32_t saddr, uint32_t lead) {
+  return ((saddr >> 4) & 0x3FFFu) | (((lead >> 4) & 0x3FFFu) << 16);
 }
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);   // atom, version, 128-byte swizzle
 
-// Tile t of the walk: channel tiles fastest inside bands of 16, so that concurrent CTAs share both
-// operands through L2.
+// Tile t of the walk: channel tiles fastest inside bands of kBand, so that concurrent CTAs share
+// both operands through L2.
 __device__ __forceinline__ void tile_at(const TcArgs &g, int t, int *tm, int *tn) {
-  constexpr int kBand = 16;
-  const int band = t / (kBand * g.tiles_n);
-  const int left = g.tiles_m - band * kBand;
-  const int height = left < kBand ? left : kBand;
+  const int band = g.by_band.of(t);
   const int in = t - band * kBand * g.tiles_n;
-  *tm = band * kBand + in % height;
-  *tn = in / height;
+  const bool last = (band + 1) * kBand > g.tiles_m;
+  const int across = last ? g.by_last.of(in) : in / kBand;
+  *tm = band * kBand + in - across * (last ? g.tiles_m - band * kBand : kBand);
+  *tn = across;
 }
 
 // Sixteen results of one channel, rows row0 .. row0 + 15: bias, activation, residual, store.
+struct ActOnAll {
+  float (&v)[16];
+  float slope;
+  template <int ACT>
+  __device__ __forceinline__ void operator()() const {
+    if constexpr (ACT != PT_B200_ACT_NONE)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = act_value<ACT>(v[j], slope);
+  }
+};
 template <class T>
-__device__ __forceinline__ void emit16(const TcArgs &g, float (&v)[16], int64_t chan, int64_t row0, float bias) {
-  const LinearEpi &e = g.e;
-  const int n = static_cast<int>(min(static_cast<int64_t>(16), g.rows - row0));
-  if (chan >= g.chans || n <= 0) return;
+__device__ __forceinline__ void emit16(const LinearEpi &e, float (&v)[16], int64_t chan, int64_t row0, int n,
+                                       float bias) {
   float r[16];
   if (e.residual) {
     const T *p = static_cast<const T *>(e.residual) + row0 * e.ldr + chan;
@@ -114,10 +227,7 @@ __device__ __forceinline__ void emit16(const TcArgs &g, float (&v)[16], int64_t 
     for (int j = 0; j < 16; ++j)
       if (j < n) p[j * e.ldp] = from_f32<T>(v[j]);
   }
-  if (e.act) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = act_value(v[j], e.act, e.slope);
-  }
+  with_act(e.act, ActOnAll{v, e.slope});
   if (e.residual) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] += r[j];
@@ -127,9 +237,8 @@ __device__ __forceinline__ void emit16(const TcArgs &g, float (&v)[16], int64_t 
   for (int j = 0; j < 16; ++j)
     if (j < n) p[j * e.ldy] = from_f32<T>(v[j]);
 }
-
-// P planes per operand, KB elements of k per stage.
-template <class T, int P, int KB>
+// G CTAs to a tile, P planes per operand.
+template <class T, int G, int P>
 __global__ void __launch_bounds__(kTcThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                      const TcArgs g, uint32_t *gerr) {
@@ -138,18 +247,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *gbase = smem_raw + (base - raw);
-  const uint32_t a_plane = kM * KB * 2, b_plane = static_cast<uint32_t>(g.bn) * KB * 2;
-  const uint32_t stage_bytes = P * (a_plane + b_plane);
+  const int b_rows = g.bn / G;                     // rows of B in this CTA
+  const uint32_t a_plane = kM * KB * 2, b_plane = static_cast<uint32_t>(b_rows) * KB * 2;
+  const uint32_t stage_bytes = (P * (a_plane + b_plane) + 1023u) & ~1023u;
   const uint32_t bar0 = base + kSmemBudget;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
   auto acc_full = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
-  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 2 + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 2 + b); };   // rank 0's counts
   const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 4);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gbase + kSmemBudget + 8 * (2 * kMaxStages + 5));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // accumulators are a power of two of columns apart, TMEM is allocated in powers of two from 32
   uint32_t acc_cols = 16;
   while (acc_cols < static_cast<uint32_t>(g.bn)) acc_cols *= 2;
@@ -157,12 +267,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < g.stages; ++s) {
-      mbar_init(full(s), 1);
+      mbar_init(full(s), 2);
       mbar_init(empty(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), kEpiWarps);
+      mbar_init(acc_empty(b), G * kEpiWarps);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -173,55 +283,81 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     prefetch_tmap(&map_b);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), tmem_cols);
-    tmem_relinquish();
+    alloc<G>(smem_u32(tmem_slot), tmem_cols);
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (G == 2) cg::this_cluster().sync();   // the other CTA's barriers are ready too
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
 
-  const int rank = static_cast<int>(blockIdx.x) % g.split;
-  const int step = static_cast<int>(gridDim.x) / g.split;
+  // What follows reads and writes global memory: after the kernels before this one.
+  if (!g.beside) wait_for_previous();
+  let_next_start();
+
+  // The CTAs of a cluster work on a tile together: the pair, or those that share its k range.
+  int rank, first, step;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %%clusterid.x;" : "=r"(first));
+  asm("mov.u32 %0, %%nclusterid.x;" : "=r"(step));
   const int tiles = g.tiles_m * g.tiles_n;
-  const int k_lo = rank * g.per, k_hi = min(k_lo + g.per, g.kiters);
-  // stages per accumulator: all of them, or (three planes) a chunk of 64 elements of k
-  const int chunk = P == 1 ? g.per : 64 / KB;
+  const int pair_rank = G == 2 ? rank : 0;
+  const int k_rank = G == 2 ? 0 : rank;
+  const int k_lo = k_rank * g.per, k_hi = min(k_lo + g.per, g.kiters);
+  // stages per accumulator: all of them, or (three planes) one
+  const int chunk = P == 1 ? g.per : 1;
 
-  if (warp == 0 && lane == 0) {
-    // ---------------- TMA producer
+  if (warp == 0 || warp == 2) {
+    // ---------------- TMA producers: A in warp 0, B in warp 2 (a copy takes 80 to 120 clocks to issue)
+    const bool is_a = warp == 0;
+    const bool one = elect_one();
     int s = 0, issued = 0;
-    uint32_t phase = 0;
+    uint32_t phase = 0, a0 = is_a ? base : base + P * a_plane;
+    const uint32_t plane = is_a ? a_plane : b_plane;
+    // a pair's copies all count on rank 0's barrier, where the MMAs are issued
+    const uint32_t bar0_of = G == 1 ? full(0) : in_rank0(full(0));
     bool ok = true;
-    for (int t = blockIdx.x / g.split; t < tiles && ok; t += step) {
+    for (int t = first; t < tiles && ok; t += step) {
       int tm, tn;
       tile_at(g, t, &tm, &tn);
+      const int chan0 = uniform((tm * G + pair_rank) * kM), row0 = uniform(tn * g.bn + pair_rank * b_rows);
       for (int k = k_lo; k < k_hi; ++k) {
         if (issued >= g.stages && !mbar_wait(empty(s), phase ^ 1u, abort_flag, gerr, ERR_WAIT_EMPTY)) {
           ok = false;
           break;
         }
-        const uint32_t a0 = base + s * stage_bytes, b0 = a0 + P * a_plane;
-        mbar_expect_tx(full(s), stage_bytes);
-        for (int p = 0; p < P; ++p) {
-          if (g.a_mn) {
-            for (int i = 0; i < kM / 64; ++i)
-              tma_load_3d(a0 + p * a_plane + i * KB * 128, &map_a, full(s), tm * kM + i * 64, k * KB, p);
+        const uint32_t bar = uniform(bar0_of + 8u * s), own = uniform(full(s));
+        const int ku = uniform(k * KB);
+        uint32_t at = uniform(a0);
+        if (one) {
+          if (pair_rank == 0) mbar_expect_tx(own, G * P * plane);
+          if (is_a) {
+#pragma unroll
+            for (int p = 0; p < P; ++p, at += a_plane) {
+              if (g.a_mn) {
+#pragma unroll
+                for (int i = 0; i < kM / 64; ++i) load<G>(at + i * KB * 128, &map_a, bar, chan0 + i * 64, ku, p);
+              } else {
+                load<G>(at, &map_a, bar, ku, chan0, p);
+              }
+            }
           } else {
-            tma_load_3d(a0 + p * a_plane, &map_a, full(s), k * KB, tm * kM, p);
-          }
-          if (g.b_mn) {
-            for (int i = 0; i < g.bn / 64; ++i)
-              tma_load_3d(b0 + p * b_plane + i * KB * 128, &map_b, full(s), tn * g.bn + i * 64, k * KB, p);
-          } else {
-            tma_load_3d(b0 + p * b_plane, &map_b, full(s), k * KB, tn * g.bn, p);
+#pragma unroll
+            for (int p = 0; p < P; ++p, at += b_plane) {
+              if (g.b_mn) {
+                for (int i = 0; i < b_rows / 64; ++i) load<G>(at + i * KB * 128, &map_b, bar, row0 + i * 64, ku, p);
+              } else {
+                load<G>(at, &map_b, bar, ku, row0, p);
+              }
+            }
           }
         }
         ++issued;
-        if (++s == g.stages) s = 0, phase ^= 1u;
+        a0 += stage_bytes;
+        if (++s == g.stages) s = 0, phase ^= 1u, a0 -= g.stages * stage_bytes;
       }
     }
-    if (!ok) {   // copies in flight must land before the CTA's shared memory is given up
+    if (!ok && pair_rank == 0 && is_a) {   // copies in flight must land before shared memory is given up
       const int flying = min(issued, g.stages);
       for (int i = 0; i < flying; ++i) {
         if (s == 0) s = g.stages, phase ^= 1u;
@@ -229,71 +365,97 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint32_t it = 0;
         while (!mbar_try_wait(full(s), phase) && ++it < kWaitLimit) {
         }
-        if (it >= kWaitLimit) atomicOr(gerr, ERR_WAIT_DRAIN);
+        if (it >= kWaitLimit && one) atomicOr(gerr, ERR_WAIT_DRAIN);
       }
     }
-  } else if (warp == 1 && lane == 0) {
-    // ---------------- MMA issuer
-    constexpr uint32_t kSwz = KB == 64 ? 2u : 4u;              // 128- or 64-byte swizzle, K-major
-    constexpr uint32_t kAtom = KB * 16;                        // 8 rows of KB elements
-    const uint32_t a_adv = g.a_mn ? 2048u >> 4 : 32u >> 4;     // 16 elements of k further on
-    const uint32_t b_adv = g.b_mn ? 2048u >> 4 : 32u >> 4;
-    int s = 0, unit = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int t = blockIdx.x / g.split; t < tiles && ok; t += step) {
-      for (int k = k_lo; k < k_hi && ok; ++unit) {
-        const int b = unit & 1;
-        if (unit >= 2 && !mbar_wait(acc_empty(b), ((unit >> 1) & 1) ^ 1u, abort_flag, gerr, ERR_WAIT_ACC)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem + b * acc_cols;
-        const int k_end = min(k + chunk, k_hi);
-        uint32_t accumulate = 0;
-        for (; k < k_end; ++k) {
-          if (!mbar_wait(full(s), phase, abort_flag, gerr, ERR_WAIT_FULL)) {
+  } else if (warp == 1) {
+    if (pair_rank == 0) {
+      // ---------------- MMA issuer
+      const bool one = elect_one();
+      const uint32_t a_adv = g.a_mn ? 2048u >> 4 : 32u >> 4;     // 16 elements of k further on
+      const uint32_t b_adv = g.b_mn ? 2048u >> 4 : 32u >> 4;
+      const uint32_t da0 = sdesc_lo(base, g.a_mn ? KB * 128 : 16);
+      const uint32_t db0 = sdesc_lo(base + P * a_plane, g.b_mn ? KB * 128 : 16);
+      int s = 0, unit = 0;
+      uint32_t phase = 0, at = 0;    // `at`: the stage's place, in the descriptors' 16 bytes
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        for (int k = k_lo; k < k_hi && ok; ++unit) {
+          const int b = unit & 1;
+          if (unit >= 2 && !mbar_wait(acc_empty(b), ((unit >> 1) & 1) ^ 1u, abort_flag, gerr, ERR_WAIT_ACC)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a0 = base + s * stage_bytes, b0 = a0 + P * a_plane;
-#pragma unroll
-          for (int q = 0; q < (P == 1 ? 1 : 6); ++q) {
-            constexpr int kPa[6] = {2, 0, 1, 1, 0, 0}, kPb[6] = {0, 2, 1, 0, 1, 0};
-            const uint32_t ap = a0 + (P == 1 ? 0 : kPa[q]) * a_plane, bp = b0 + (P == 1 ? 0 : kPb[q]) * b_plane;
-            const uint64_t da = g.a_mn ? sdesc(ap, KB * 128, 1024, 2) : sdesc(ap, 16, kAtom, kSwz);
-            const uint64_t db = g.b_mn ? sdesc(bp, KB * 128, 1024, 2) : sdesc(bp, 16, kAtom, kSwz);
-#pragma unroll
-            for (int i = 0; i < KB / 16; ++i) {
-              mma_f16(d, da + i * a_adv, db + i * b_adv, g.idesc, accumulate);
-              accumulate = 1;
+          const uint32_t d = uniform(tmem + b * acc_cols);
+          const int k_end = min(k + chunk, k_hi);
+          uint32_t accumulate = 0;
+          for (; k < k_end; ++k) {
+            if (!mbar_wait(full(s), phase, abort_flag, gerr, ERR_WAIT_FULL)) {
+              ok = false;
+              break;
             }
+            tc_fence_after();
+            const uint32_t here = uniform(at), first_of = uniform(accumulate), free_bar = uniform(empty(s));
+            if (one) {
+#pragma unroll
+              for (int q = 0; q < (P == 1 ? 1 : 6); ++q) {
+                constexpr int kPa[6] = {2, 0, 1, 1, 0, 0}, kPb[6] = {0, 2, 1, 0, 1, 0};
+                const uint32_t da = da0 + here + (P == 1 ? 0 : kPa[q]) * (a_plane >> 4);
+                const uint32_t db = db0 + here + (P == 1 ? 0 : kPb[q]) * (b_plane >> 4);
+                if (q == 0)
+                  mma_f16<G, true>(d, da, db, kDescHi, g.idesc, first_of);
+                else
+                  mma_f16<G, false>(d, da, db, kDescHi, g.idesc, 1);
+#pragma unroll
+                for (int i = 1; i < KB / 16; ++i)
+                  mma_f16<G, false>(d, da + i * a_adv, db + i * b_adv, kDescHi, g.idesc, 1);
+              }
+              commit<G>(free_bar);
+            }
+            accumulate = 1;
+            at += stage_bytes >> 4;
+            if (++s == g.stages) s = 0, phase ^= 1u, at = 0;
           }
-          mma_commit(empty(s));
-          if (++s == g.stages) s = 0, phase ^= 1u;
+          if (ok && one) commit<G>(acc_full(b));
         }
-        if (ok) mma_commit(acc_full(b));
+      }
+      if (!ok) {   // MMAs already issued must finish before TMEM is released
+        if (one) commit<G>(drain);
+        uint32_t it = 0;
+        while (!mbar_try_wait(drain, 0) && ++it < kWaitLimit) {
+        }
+        if (it >= kWaitLimit && one) atomicOr(gerr, ERR_WAIT_DRAIN);
       }
     }
-    if (!ok) {   // MMAs already issued must finish before TMEM is released
-      mma_commit(drain);
-      uint32_t it = 0;
-      while (!mbar_try_wait(drain, 0) && ++it < kWaitLimit) {
-      }
-      if (it >= kWaitLimit) atomicOr(gerr, ERR_WAIT_DRAIN);
-    }
-  } else if (warp >= 4) {
-    // ---------------- epilogue warps: lanes 32 (warp % 4) .. + 31, every other block of 16 columns
-    const int quad = warp & 3, half = (warp - 4) >> 2;
+  } else {
+    // ---------------- epilogue warps: lanes 32 (warp % 4) .. + 31, every fourth block of 16 columns
+    const int quad = warp & 3, half = (warp - kFirstEpi) >> 2;
     const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    if (g.sums.parts > 0 && warp < kFirstEpi + kSumLanes) {   // column sums, 32 columns at a time, while the first tile's products run
+      float *red = reinterpret_cast<float *>(gbase + kSmemBudget + 512);
+      const int row = warp - kFirstEpi;
+      for (int64_t c0 = blockIdx.x * 32; c0 < g.sums.n; c0 += gridDim.x * 32) {
+        float v = 0.0f;
+        if (c0 + lane < g.sums.n)
+#pragma unroll 4
+          for (int p = row; p < g.sums.parts; p += kSumLanes) v += g.sums.part[p * g.sums.n + c0 + lane];
+        red[row * 33 + lane] = v;
+        asm volatile("bar.sync 1, %0;" ::"n"(kSumLanes * 32) : "memory");
+        if (row == 0 && c0 + lane < g.sums.n) {
+          v = 0.0f;
+          for (int i = 0; i < kSumLanes; ++i) v += red[i * 33 + lane];
+          static_cast<T *>(g.sums.out)[c0 + lane] = from_f32<T>(v);
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kSumLanes * 32) : "memory");
+      }
+    }
     int unit = 0;
     bool ok = true;
-    for (int t = blockIdx.x / g.split; t < tiles && ok; t += step) {
+    for (int t = first; t < tiles && ok; t += step) {
       int tm, tn;
       tile_at(g, t, &tm, &tn);
-      const int64_t chan = static_cast<int64_t>(tm) * kM + quad * 32 + lane;
+      const int64_t chan = static_cast<int64_t>(tm * G + pair_rank) * kM + quad * 32 + lane;
       const int64_t row0 = static_cast<int64_t>(tn) * g.bn;
       const float bias = g.e.bias && chan < g.chans ? to_f32(static_cast<const T *>(g.e.bias)[chan]) : 0.0f;
       float *part = reinterpret_cast<float *>(gbase);   // split: [bn][128] of this CTA's part
@@ -301,24 +463,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int b = unit & 1;
         if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC)) break;
         tc_fence_after();
-        for (int c = half * 16; c < g.bn; c += 32) {
+        for (int c = half * 16; c < g.bn; c += 64) {
           float v[16];
           tmem_ld16(tl + b * acc_cols + c, v);
           if (g.split > 1) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) part[(c + j) * kM + quad * 32 + lane] = v[j];
           } else {
-            emit16<T>(g, v, chan, row0 + c, bias);
+            const int n = static_cast<int>(min(static_cast<int64_t>(16), g.rows - row0 - c));
+            if (chan < g.chans && n > 0) emit16<T>(g.e, v, chan, row0 + c, n, bias);
           }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty(b));
+        if (lane == 0) arrive<G>(G == 1 ? acc_empty(b) : in_rank0(acc_empty(b)));
         ++unit;
       } else {
-        float acc[8][16];
+        float acc[kMaxBn3 / 64][16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kMaxBn3 / 64; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
         for (int k = k_lo; k < k_hi && ok; k += chunk, ++unit) {
@@ -329,53 +492,64 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (half * 16 + i * 32 < g.bn) {
+          for (int i = 0; i < kMaxBn3 / 64; ++i) {
+            if (half * 16 + i * 64 < g.bn) {
               float v[16];
-              tmem_ld16(tl + b * acc_cols + half * 16 + i * 32, v);
+              tmem_ld16(tl + b * acc_cols + half * 16 + i * 64, v);
 #pragma unroll
               for (int j = 0; j < 16; ++j) acc[i][j] += v[j];
             }
           }
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(acc_empty(b));
+          if (lane == 0) arrive<G>(G == 1 ? acc_empty(b) : in_rank0(acc_empty(b)));
         }
         if (!ok) break;
         if (g.split > 1) {
           // the stages still hold operands of the last chunk until its MMAs are done, which the
           // last accumulator's arrival says
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (half * 16 + i * 32 < g.bn)
+          for (int i = 0; i < kMaxBn3 / 64; ++i)
+            if (half * 16 + i * 64 < g.bn)
 #pragma unroll
               for (int j = 0; j < 16; ++j)
-                part[(half * 16 + i * 32 + j) * kM + quad * 32 + lane] = acc[i][j];
+                part[(half * 16 + i * 64 + j) * kM + quad * 32 + lane] = acc[i][j];
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (half * 16 + i * 32 < g.bn) emit16<T>(g, acc[i], chan, row0 + half * 16 + i * 32, bias);
+          for (int i = 0; i < kMaxBn3 / 64; ++i) {
+            const int c = half * 16 + i * 64;
+            const int n = static_cast<int>(min(static_cast<int64_t>(16), g.rows - row0 - c));
+            if (c < g.bn && chan < g.chans && n > 0) {
+              emit16<T>(g.e, acc[i], chan, row0 + c, n, bias);
+            }
+          }
         }
       }
     }
   }
-  if (g.split > 1) {
+  __syncwarp();
+  if (G == 1 && g.split > 1) {
     // ---------------- one tile per cluster: add the parts, a slice of the rows per CTA
-    __syncwarp();
     auto cluster = cg::this_cluster();
     cluster.sync();
-    const int t = blockIdx.x / g.split;
-    if (warp >= 4 && !*abort_flag) {
-      const int quad = warp & 3, half = (warp - 4) >> 2;
+    if (warp >= kFirstEpi && !*abort_flag) {
+      const int quad = warp & 3, half = (warp - kFirstEpi) >> 2;
       int tm, tn;
-      tile_at(g, t, &tm, &tn);
+      tile_at(g, first, &tm, &tn);
       const int64_t chan = static_cast<int64_t>(tm) * kM + quad * 32 + lane;
       float *part = reinterpret_cast<float *>(gbase);
       const int width = g.bn / g.split;
-      for (int c = rank * width + half; c < (rank + 1) * width; c += 2) {
+      const float *from[kMaxSplit];
+#pragma unroll
+      for (int r = 0; r < kMaxSplit; ++r)
+        from[r] = cluster.map_shared_rank(part, r < g.split ? r : 0) + quad * 32 + lane;
+      for (int c = rank * width + half; c < (rank + 1) * width; c += 4) {
         const int64_t row = static_cast<int64_t>(tn) * g.bn + c;
-        float v = 0.0f;
-        for (int r = 0; r < g.split; ++r) v += cluster.map_shared_rank(part, r)[c * kM + quad * 32 + lane];
+        float got[kMaxSplit], v = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kMaxSplit; ++r) got[r] = r < g.split ? from[r][c * kM] : 0.0f;
+#pragma unroll
+        for (int r = 0; r < kMaxSplit; ++r) v += got[r];
         if (chan < g.chans && row < g.rows) linear_store<T>(g.e, row, chan, v);
       }
     }
@@ -383,35 +557,131 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (G == 2) cg::this_cluster().sync();   // nor while the pair's MMAs or arrivals reach it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, tmem_cols);
+    dealloc<G>(tmem, tmem_cols);
+  }
+  // a kernel that ran beside the one before it ends after it: the next may wait for this one alone
+  if (g.beside) wait_for_previous();
+}
+
+// ------------------------------------------------------------------------------ operand passes
+constexpr int kPrepBlock = 256;
+constexpr int kPrepRows = 2;   // rows a thread has in flight
+
+template <class T>
+struct Eight {
+  T v[8];
+};
+template <class T>
+__device__ __forceinline__ void load8(const T *p, int n, bool vec, Eight<T> *o) {
+  if (vec) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8 / V; ++i)
+      *reinterpret_cast<Pack<T, V> *>(o->v + i * V) = *reinterpret_cast<const Pack<T, V> *>(p + i * V);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o->v[i] = i < n ? p[i] : from_f32<T>(0.0f);
   }
 }
 
-// ------------------------------------------------------------------------------ operand planes
-// A matrix copied into the rows and planes the tensor cores read.
+// One thread's rows of a job: eight columns of every `step`-th row from r0.
 template <class T>
-__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
-  const int64_t cols8 = a.ld_out;
-  const int64_t total = a.rows * cols8;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = i / cols8, c = i % cols8;
-    if (c >= a.cols) continue;
-    const T v = static_cast<const T *>(a.src)[r * a.ld + c];
-    if constexpr (sizeof(T) == 4) {
-      __nv_bfloat16 o[3];
-      split3(v, o);
+struct PrepRows {
+  const PrepJob &a;
+  int64_t c, r0, step;
+  int n;
+  float (&sum)[8];
+  template <int ACT>
+  __device__ __forceinline__ void operator()() const {
+    for (int64_t r1 = r0; r1 < a.rows; r1 += kPrepRows * step) {
+      Eight<T> s[kPrepRows], p[kPrepRows];
 #pragma unroll
-      for (int p = 0; p < 3; ++p) static_cast<__nv_bfloat16 *>(a.dst)[p * a.plane + i] = o[p];
-    } else {
-      static_cast<T *>(a.dst)[i] = v;
+      for (int u = 0; u < kPrepRows; ++u) {
+        const int64_t r = r1 + u * step;
+        if (r < a.rows) {
+          load8(static_cast<const T *>(a.src) + r * a.ld + c, n, a.vec, &s[u]);
+          if constexpr (ACT != PT_B200_ACT_NONE)
+            load8(static_cast<const T *>(a.pre) + r * a.ldp + c, n, a.vec, &p[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kPrepRows; ++u) {
+        const int64_t r = r1 + u * step;
+        if (r >= a.rows) break;
+        float d[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          d[i] = to_f32(s[u].v[i]);
+          // (explicit operations: a sum must not depend on what else is made of d)
+          if constexpr (ACT != PT_B200_ACT_NONE)
+            d[i] = __fmul_rn(d[i], act_grad<ACT>(to_f32(p[u].v[i]), a.slope));
+          sum[i] = __fadd_rn(sum[i], d[i]);
+        }
+        if (!a.dst) continue;
+        if constexpr (sizeof(T) == 4) {
+          Pack<__nv_bfloat16, 8> o[3];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            __nv_bfloat16 q[3];
+            split3(d[i], q);
+            o[0].v[i] = q[0];
+            o[1].v[i] = q[1];
+            o[2].v[i] = q[2];
+          }
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            *reinterpret_cast<Pack<__nv_bfloat16, 8> *>(static_cast<__nv_bfloat16 *>(a.dst) + i * a.plane +
+                                                        r * a.ldd + c) = o[i];
+        } else {
+          // rounded to the operands' type for the products; the sums take the fp32 value
+          Pack<T, 8> o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o.v[i] = from_f32<T>(d[i]);
+          *reinterpret_cast<Pack<T, 8> *>(static_cast<T *>(a.dst) + r * a.ldd + c) = o;
+        }
+      }
     }
   }
+};
+
+// Bound by HBM: src and pre are read once and dst is written once, 16 bytes a thread at a time
+// where rows are aligned.
+template <class T>
+__global__ void __launch_bounds__(kPrepBlock, 3) prep_kernel(const __grid_constant__ PrepJobs jobs) {
+  __shared__ float red[kPrepBlock * 8];
+  let_next_start();
+  int job = 0, block = blockIdx.x;
+#pragma unroll
+  for (int i = 0; i < kMaxJobs - 1; ++i)
+    if (static_cast<int>(blockIdx.x) >= jobs.end[i]) job = i + 1, block = blockIdx.x - jobs.end[i];
+  const PrepJob &a = jobs.j[job];
+  const int tx = threadIdx.x & (a.lanes - 1), ty = threadIdx.x / a.lanes, height = kPrepBlock / a.lanes;
+  const int cb = block % a.col_blocks, rb = block / a.col_blocks;
+  const int64_t c = (static_cast<int64_t>(cb) * a.lanes + tx) * 8;
+  const int n = static_cast<int>(min(static_cast<int64_t>(8), a.cols - c));
+  float sum[8] = {};
+  if (n > 0)
+    with_act(a.act, PrepRows<T>{a, c, static_cast<int64_t>(rb) * height + ty,
+                                static_cast<int64_t>(a.row_blocks) * height, n, sum});
+  if (!a.part) return;
+  // the block's row lanes, added in order
+  const int width = a.lanes * 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[ty * width + tx * 8 + i] = sum[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < width; i += kPrepBlock) {
+    const int64_t col = static_cast<int64_t>(cb) * width + i;
+    if (col >= a.cols) break;
+    float v = 0.0f;
+    for (int k = 0; k < height; ++k) v += red[k * width + i];
+    a.part[static_cast<int64_t>(rb) * a.cols + col] = v;
+  }
 }
 
-int encode(CUtensorMap *m, const TcOperand &o, bool half, int planes, int box_inner, int box_outer, bool swz64) {
+int encode(CUtensorMap *m, const TcOperand &o, bool half, int planes, int box_inner, int box_outer) {
   PFN_cuTensorMapEncodeTiled_v12000 enc;
   if (tensor_map_encoder(&enc)) return -1;
   cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)planes};
@@ -420,83 +690,104 @@ int encode(CUtensorMap *m, const TcOperand &o, bool half, int planes, int box_in
   cuuint32_t es[3] = {1, 1, 1};
   const CUresult r = enc(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                          const_cast<void *>(o.p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         swz64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   PTB_REQUIRE(r == CUDA_SUCCESS, "pt_b200: operand tensor map encode failed (%d)", (int)r);
   return 0;
 }
 
-// Tile height and k split: the cheapest of the candidates by a count of SM clocks.  A stage of 64
-// elements of k takes the longer of its MMAs (bn / 2 clocks for 16 of k) and of its bytes at the
-// L2's share of one SM; a tile adds its start, its epilogue and, when its k range is shared, the
-// exchange of the parts.
+// CTAs to a tile, rows per tile and k split: the cheapest of the candidates by a count of SM
+// clocks, whose figures are measurements (B200, clocks read in the kernel at 64 of k a stage):
+//   - an MMA of 16 of k takes bn / 2 clocks, or what its operands take to leave shared memory at
+//     128 bytes a clock (4 KB of A, and B's rows of this CTA), next to the copies that fill it;
+//   - a stage's bytes arrive at about 75 a clock (the L2's rate when all SMs ask: bf16 pairs of
+//     128 rows 319 clocks a stage, of 224 rows 398), and no stage takes less than 330;
+//   - a tile starts after 2800 and leaves after 300 + 15 bn, which the next tile hides;
+//   - parts of a split tile are exchanged in 3500 + 4 bn.
+// The clusters of a split must fit the GPU at once.
 struct Shape {
-  int bn, split;
+  int group, bn, split;
 };
-Shape pick_shape(int sms, int64_t rows, int64_t chans, int kiters, int kb, int planes, bool b_mn) {
-  Shape best{0, 1};
+Shape pick_shape(const pt_b200_ops *h, int64_t rows, int64_t chans, int kiters, int planes, bool b_mn) {
+  Shape best{0, 0, 1};
   double best_cost = 0;
-  const int64_t tm = (chans + kM - 1) / kM;
   const int products = planes == 1 ? 1 : 6;
-  for (int bn : {16, 32, 64, 128, 256}) {
-    if (b_mn && bn < 64) continue;
-    const int64_t tiles = tm * ((rows + bn - 1) / bn);
-    for (int split : {1, 2, 4, 8}) {
-      const int per = (kiters + split - 1) / split;
-      if (split > 1 && ((split - 1) * per >= kiters || tiles * split > sms)) continue;
-      const double mma = products * (kb / 16) * std::max(bn / 2.0, 16.0);
-      const double load = planes * kb * 2.0 * (kM + bn) / 60.0;
-      const double tail = 600.0 + bn * (split > 1 ? 8.0 + 6.0 * split : 8.0);
-      const int64_t waves = (tiles * split + sms - 1) / sms;
-      const double cost = 2000.0 + waves * (per * std::max(mma, load)) + tail;
-      if (!best.bn || cost < best_cost) best = Shape{bn, split}, best_cost = cost;
+  for (int group : {1, 2}) {
+    const int64_t tm = (chans + group * kM - 1) / (group * kM);
+    for (int bn = 16; bn <= (planes == 1 ? kMaxBn1 : kMaxBn3); bn += 16) {
+      // an MN-major tile is made of blocks of 64; accumulators of a pair start at 32 rows
+      if ((b_mn && bn % (64 * group)) || (group == 2 && bn % 32)) continue;
+      const double bytes = planes * KB * 2.0 * (kM + bn / group);
+      if (2 * bytes > kSmemBudget) continue;   // two stages at least
+      const int mmas = products * (KB / 16);
+      const double stage = std::max(std::max(mmas * bn / 2.0, mmas * (32 + bn / (4.0 * group)) + bytes * 0.6 / 128),
+                                    std::max(bytes / 75, 330.0));
+      const double leave = 300 + 15.0 * bn;
+      const int64_t tiles = tm * ((rows + bn - 1) / bn);
+      for (int split = 1, log = 0; split <= kMaxSplit; split *= 2, ++log) {
+        const int per = (kiters + split - 1) / split;
+        if (split > 1 && (group == 2 || (split - 1) * per >= kiters || tiles > h->clusters[log])) continue;
+        const int64_t at_once = group == 2 ? h->clusters[1] : h->clusters[log];
+        const int64_t waves = (tiles + at_once - 1) / at_once;
+        const double cost = 2800 + waves * std::max(per * stage, leave) + leave + (split > 1 ? 3500 + 4.0 * bn : 0);
+        if (!best.bn || cost < best_cost) best = Shape{group, bn, split}, best_cost = cost;
+      }
     }
   }
   return best;
 }
 
-template <class T, int P, int KB>
-int launch(const pt_b200_ops *h, const TcProduct &p, cudaStream_t st) {
+template <class T, int P>
+int launch(const pt_b200_ops *h, const TcProduct &p, const ColumnSums &sums, bool early, bool beside,
+           cudaStream_t st) {
   TcArgs g{};
+  g.sums = sums;
+  g.beside = beside;
   g.e = p.e;
   g.rows = p.rows;
   g.chans = p.chans;
   g.a_mn = p.a_mn;
   g.b_mn = p.b_mn;
   g.kiters = static_cast<int>((p.k + KB - 1) / KB);
-  const Shape sh = pick_shape(h->sms, p.rows, p.chans, g.kiters, KB, P, p.b_mn);
+  const Shape sh = pick_shape(h, p.rows, p.chans, g.kiters, P, p.b_mn);
+  const int G = sh.group;
   g.bn = sh.bn;
   g.split = sh.split;
   g.per = (g.kiters + g.split - 1) / g.split;
-  const int stage = P * (kM + g.bn) * KB * 2;
+  const int stage = static_cast<int>(round_up(P * (kM + g.bn / G) * KB * 2, 1024));
   g.stages = std::min(kMaxStages, kSmemBudget / stage);
-  g.tiles_m = static_cast<int>((p.chans + kM - 1) / kM);
+  g.tiles_m = static_cast<int>((p.chans + G * kM - 1) / (G * kM));
   const int64_t tiles_n = (p.rows + g.bn - 1) / g.bn;
-  PTB_REQUIRE(tiles_n * g.tiles_m < (int64_t(1) << 30), "pt_b200: product of %lld x %lld is too large",
+  PTB_REQUIRE(tiles_n * g.tiles_m < (int64_t(1) << 29), "pt_b200: product of %lld x %lld is too large",
               (long long)p.rows, (long long)p.chans);
   g.tiles_n = static_cast<int>(tiles_n);
   constexpr bool kHalf = std::is_same_v<T, __half>;
   const uint32_t fmt = kHalf ? 0u : 1u;
   g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u) |
-            (static_cast<uint32_t>(g.bn >> 3) << 17) | (static_cast<uint32_t>(kM >> 4) << 24);
+            (static_cast<uint32_t>(g.bn >> 3) << 17) | (static_cast<uint32_t>(G * kM >> 4) << 24);
   CUtensorMap ma, mb;
-  if (encode(&ma, p.a, kHalf, P, p.a_mn ? 64 : KB, p.a_mn ? KB : kM, !p.a_mn && KB == 32) ||
-      encode(&mb, p.b, kHalf, P, p.b_mn ? 64 : KB, p.b_mn ? KB : g.bn, !p.b_mn && KB == 32))
+  if (encode(&ma, p.a, kHalf, P, p.a_mn ? 64 : KB, p.a_mn ? KB : kM) ||
+      encode(&mb, p.b, kHalf, P, p.b_mn ? 64 : KB, p.b_mn ? KB : g.bn / G))
     return -1;
-  auto kernel = linear_tc_kernel<T, P, KB>;
-  PTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  auto kernel = G == 1 ? linear_tc_kernel<T, 1, P> : linear_tc_kernel<T, 2, P>;
+  g.by_band = Divide(static_cast<uint32_t>(kBand * g.tiles_n));
+  g.by_last = Divide(g.tiles_m % kBand ? g.tiles_m % kBand : kBand);
   const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
+  const int group = G * g.split;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(g.split > 1 ? tiles * g.split : std::min<int64_t>(tiles, h->sms)));
+  const int64_t at_once = group == 1 ? h->clusters[0] : group == 2 ? h->clusters[1] : tiles;
+  cfg.gridDim = dim3(static_cast<unsigned>(group * std::min(tiles, at_once)));
   cfg.blockDim = dim3(kTcThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = g.split;
+  at[0].val.clusterDim.x = group;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = early ? 2 : 1;
   PTB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, g, h->gerr));
   count_launch();
   return 0;
@@ -505,6 +796,33 @@ int launch(const pt_b200_ops *h, const TcProduct &p, cudaStream_t st) {
 }  // namespace
 
 namespace ptb {
+
+int tc_setup(pt_b200_ops *h) {
+  const void *const kernels[] = {
+      reinterpret_cast<const void *>(linear_tc_kernel<float, 1, 3>),
+      reinterpret_cast<const void *>(linear_tc_kernel<float, 2, 3>),
+      reinterpret_cast<const void *>(linear_tc_kernel<__nv_bfloat16, 1, 1>),
+      reinterpret_cast<const void *>(linear_tc_kernel<__nv_bfloat16, 2, 1>),
+      reinterpret_cast<const void *>(linear_tc_kernel<__half, 1, 1>),
+      reinterpret_cast<const void *>(linear_tc_kernel<__half, 2, 1>)};
+  for (const void *k : kernels)
+    PTB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  for (int log = 0; log < 4; ++log) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(h->sms / (1 << log) << log));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = kSmemBytes;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 1 << log;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    PTB_CUDA(cudaOccupancyMaxActiveClusters(&h->clusters[log], kernels[log == 1 ? 1 : 0], &cfg));
+    PTB_REQUIRE(h->clusters[log] > 0, "pt_b200: no cluster of %d blocks fits this GPU", 1 << log);
+  }
+  return 0;
+}
 
 int64_t tc_plane_bytes(int dtype, int64_t rows, int64_t cols) {
   const int64_t ld = round_up(cols, 8);
@@ -524,22 +842,51 @@ TcOperand tc_tensor(const void *p, int64_t rows, int64_t cols, int64_t ld) {
   return TcOperand{p, rows, cols, rows == 1 ? round_up(cols, 8) : ld, 0};
 }
 
-int tc_pack(const pt_b200_ops *h, int dtype, const void *src, int64_t ld, const TcOperand &to, cudaStream_t st) {
-  const PackArgs a{src, const_cast<void *>(to.p), to.rows, to.cols, ld, to.ld, to.plane};
-  const int64_t blocks = std::min<int64_t>((to.rows * to.ld + 255) / 256, static_cast<int64_t>(h->sms) * 16);
+static int prep_lanes(int64_t cols) {
+  int lanes = 1;
+  while (lanes < 32 && lanes * 8 < cols) lanes *= 2;
+  return lanes;
+}
+
+int tc_row_blocks(const pt_b200_ops *h, int64_t rows, int64_t cols) {
+  const int lanes = prep_lanes(cols), height = kPrepBlock / lanes;
+  const int64_t col_blocks = (cols + lanes * 8 - 1) / (lanes * 8);
+  const int64_t want = (rows + height * kPrepRows - 1) / (height * kPrepRows);
+  const int64_t cap = std::max<int64_t>(1, static_cast<int64_t>(h->sms) * 4 / col_blocks);
+  return static_cast<int>(std::min(want, cap));
+}
+
+void tc_add_job(const pt_b200_ops *h, int dtype, PrepJobs *jobs, int *n, PrepJob a) {
+  const int v = 16 / dtype_bytes(dtype);
+  a.lanes = prep_lanes(a.cols);
+  a.col_blocks = static_cast<int>((a.cols + a.lanes * 8 - 1) / (a.lanes * 8));
+  a.row_blocks = tc_row_blocks(h, a.rows, a.cols);
+  auto aligned = [&](const void *p, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a.rows == 1 || ld % v == 0);
+  };
+  a.vec = a.cols % 8 == 0 && aligned(a.src, a.ld) && (!a.act || aligned(a.pre, a.ldp));
+  jobs->j[*n] = a;
+  const int first = *n ? jobs->end[*n - 1] : 0;
+  for (int i = *n; i < kMaxJobs; ++i) jobs->end[i] = first + a.col_blocks * a.row_blocks;
+  ++*n;
+}
+
+int tc_prep(int dtype, const PrepJobs &jobs, int n, cudaStream_t st) {
+  if (n == 0) return 0;
   return with_dtype(dtype, [&](auto *z) -> int {
-    pack_kernel<std::remove_pointer_t<decltype(z)>><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+    prep_kernel<std::remove_pointer_t<decltype(z)>><<<jobs.end[n - 1], kPrepBlock, 0, st>>>(jobs);
     PTB_CUDA(cudaGetLastError());
     count_launch();
     return 0;
   });
 }
 
-int tc_product(const pt_b200_ops *h, int dtype, const TcProduct &p, cudaStream_t st) {
+int tc_product(const pt_b200_ops *h, int dtype, const TcProduct &p, const ColumnSums &sums, bool early, bool beside,
+               cudaStream_t st) {
   switch (dtype) {
-    case PT_B200_F32: return launch<float, 3, 32>(h, p, st);
-    case PT_B200_BF16: return launch<__nv_bfloat16, 1, 64>(h, p, st);
-    default: return launch<__half, 1, 64>(h, p, st);
+    case PT_B200_F32: return launch<float, 3>(h, p, sums, early, beside, st);
+    case PT_B200_BF16: return launch<__nv_bfloat16, 1>(h, p, sums, early, beside, st);
+    default: return launch<__half, 1>(h, p, sums, early, beside, st);
   }
 }
 

@@ -36,18 +36,41 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&o)[3]) {
   o[2] = __float2bfloat16_rn(r1 - __bfloat162float(o[1]));
 }
 
-struct PackArgs {
-  const void *src;
+// One pass over a matrix that makes an operand of it: dst receives src * act'(pre) (src itself
+// without an activation) in the rows and planes the tensor cores read, part its column sums, one
+// row of partials per block of rows.  dst or part may be null.
+struct PrepJob {
+  const void *src, *pre;
   void *dst;
-  int64_t rows, cols, ld, ld_out, plane;
+  float *part;
+  int64_t rows, cols, ld, ldp, ldd, plane;
+  int act;
+  float slope;
+  int lanes;                   // threads across the columns, 8 columns each (a power of two)
+  int col_blocks, row_blocks;
+  bool vec;
+};
+constexpr int kMaxJobs = 3;
+struct PrepJobs {
+  PrepJob j[kMaxJobs];
+  int end[kMaxJobs];           // running count of blocks
 };
 
+// Once per handle: the kernels' shared memory, and how many of their clusters fit the GPU.
+int tc_setup(pt_b200_ops *h);
 // Whether a tensor can be read where it lies; else the bytes of its planes.
 bool tc_direct(int dtype, const void *p, int64_t rows, int64_t ld);
 int64_t tc_plane_bytes(int dtype, int64_t rows, int64_t cols);
 TcOperand tc_tensor(const void *p, int64_t rows, int64_t cols, int64_t ld);
 TcOperand tc_planes(void *p, int64_t rows, int64_t cols);
-int tc_pack(const pt_b200_ops *h, int dtype, const void *src, int64_t ld, const TcOperand &to, cudaStream_t st);
-int tc_product(const pt_b200_ops *h, int dtype, const TcProduct &p, cudaStream_t st);
+// Adds a pass to `jobs` (one launch runs them all) and gives the rows of partials it will write.
+int tc_row_blocks(const pt_b200_ops *h, int64_t rows, int64_t cols);
+void tc_add_job(const pt_b200_ops *h, int dtype, PrepJobs *jobs, int *n, PrepJob job);
+int tc_prep(int dtype, const PrepJobs &jobs, int n, cudaStream_t st);
+// After a kernel of the same call that lets it start early, `early` hides the launch behind it;
+// `sums` is work that its epilogue warps do while the first tile's products run.  With `beside` the
+// product needs nothing of the kernel right before it, only of those before that one.
+int tc_product(const pt_b200_ops *h, int dtype, const TcProduct &p, const ColumnSums &sums, bool early, bool beside,
+               cudaStream_t st);
 
 }  // namespace ptb

@@ -1,7 +1,7 @@
 // ops.cu -- the operators' handle (pt_b200_ops_*).
 #include <new>
 
-#include "ops.cuh"
+#include "linear_tc.cuh"
 
 using namespace ptb;
 
@@ -29,7 +29,13 @@ extern "C" pt_b200_ops *pt_b200_ops_create(int device) {
     set_error("pt_b200_ops_create: out of device memory");
     return nullptr;
   }
-  return new (std::nothrow) pt_b200_ops{device, prop.multiProcessorCount, gerr};
+  pt_b200_ops *h = new (std::nothrow) pt_b200_ops{device, prop.multiProcessorCount, gerr, {}};
+  if (!h || tc_setup(h)) {
+    cudaFree(gerr);
+    delete h;
+    return nullptr;
+  }
+  return h;
 }
 
 extern "C" void pt_b200_ops_destroy(pt_b200_ops *h) {
