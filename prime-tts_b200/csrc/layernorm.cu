@@ -6,17 +6,29 @@
 //   dgamma = sum over rows of dy * xhat;  dbeta = sum over rows of dy
 //
 // Both passes are bound by HBM: forward reads x and writes y once, backward reads x and dy and
-// writes dx once; the row lives in registers between its reduction and its use.  The variance is
-// the mean of the squared deviations from the mean already known (two sums over registers, not a
-// difference of two large sums).
+// writes dx once.  What that takes is enough bytes in flight while a row is being reduced: rows
+// travel through a ring of kDepth slots in shared memory (asynchronous 16-byte copies), so that the
+// next rows are on their way without holding registers.  A row of registers per thread with plain
+// loads left 8 warps on an SM and ran 16384 x 4096 bf16 at 2.4 TB/s.  The variance is the mean of
+// the squared deviations from the mean already known (two sums over registers, not a difference of
+// two large sums).
 //
-// A row is owned by TPR threads: a warp when it fits the warp's registers (no barriers, the
-// reductions are shuffles), else a block of 256.  Rows wider than kMaxRegCols are read again
-// instead of kept.  The weight gradients are column sums over all rows: each block keeps its own
-// rows' sums in registers, adds its warps' sums in shared memory and writes one row of partials,
-// and a second kernel adds the blocks' partials in their order, so that results do not depend on
-// timing.
+// With that, what bounds a 2-byte row is the instructions for it: a row's two reductions cost each of
+// its warps some 120, so a row is owned by as few threads as hold it with 32 elements each (TPR = 32
+// to 512; 8 or 16 elements in narrow rows), elements go through the arithmetic in pairs (the packed
+// fp32 instructions), and gamma and beta wait in shared memory in their own type.  32768 x 4096 bf16
+// with 16 elements on 256 threads and single arithmetic: 127 us.  Rows wider than kMaxRegCols are
+// read again instead of kept.
+//
+// Where rows are aligned a thread reads back only what it copied itself, with no barrier; where they
+// are not, the aligned 16-byte pieces that hold the row are copied (the bytes beside it are not
+// used) and every thread picks single elements.
+//
+// The weight gradients are column sums over all rows: each thread keeps its columns' sums over the
+// rows it walks; a block adds its rows' sums in shared memory and writes one row of partials, and a
+// second kernel adds the blocks' partials in a fixed order, so that results do not depend on timing.
 #include "ops.cuh"
+#include "ptx.cuh"
 
 using namespace ptb;
 
@@ -25,40 +37,88 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kMaxRegCols = 16384;
 
-// Sum of v over the TPR threads of a row (all of them get it).
+// The TPR threads of a row: a barrier, and sums that all of them get.  `red` holds 2 x 16 floats
+// that the row's previous sum did not use.
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float *red) {
+__device__ __forceinline__ void row_sync(int group) {
+  if constexpr (TPR == 32)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(TPR) : "memory");
+}
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float *red, int group) {
   v = warp_sum(v);
   if constexpr (TPR == 32) return v;
-  const int warp = threadIdx.x >> 5;
+  const int warp = (threadIdx.x % TPR) >> 5;
   if ((threadIdx.x & 31) == 0) red[warp] = v;
-  __syncthreads();
+  row_sync<TPR>(group);
   float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < TPR / 32; ++i) s += red[i];
-  __syncthreads();
   return s;
 }
-
-// Two sums with one pair of barriers.
 template <int TPR>
-__device__ __forceinline__ void row_sum2(float &a, float &b, float *red) {
+__device__ __forceinline__ void row_sum2(float &a, float &b, float *red, int group) {
   a = warp_sum(a);
   b = warp_sum(b);
   if constexpr (TPR == 32) return;
-  const int warp = threadIdx.x >> 5;
+  const int warp = (threadIdx.x % TPR) >> 5;
   if ((threadIdx.x & 31) == 0) {
     red[warp] = a;
-    red[8 + warp] = b;
+    red[16 + warp] = b;
   }
-  __syncthreads();
+  row_sync<TPR>(group);
   a = b = 0.0f;
 #pragma unroll
   for (int i = 0; i < TPR / 32; ++i) {
     a += red[i];
-    b += red[8 + i];
+    b += red[16 + i];
   }
-  __syncthreads();
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// 1 / sqrt(v): the hardware's approximation and one step of Newton's iteration, which leaves the
+// rounding of its last operations.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float y = rsqrtf(v);
+  const float e = fmaf(-v * y, y, 1.0f);
+  return isfinite(e) ? fmaf(0.5f * y, e, y) : y;   // (1 / sqrt(0) and of infinity are y itself)
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 struct NormArgs {
@@ -67,84 +127,179 @@ struct NormArgs {
   float *mean, *rstd;          // forward: written (may be null); backward: read
   float *part;                 // backward: [blocks][2][cols] partial dgamma, dbeta (may be null)
   int64_t rows, cols, ldx, lddy, ldy;
+  int pitch;                   // bytes of one row in a slot, unaligned rows
   float eps;
 };
 
-// Element j of thread t's vector i sits in column (i * TPR + t) * V + j.
-template <class T, int TPR, int V, int N>
-__global__ void __launch_bounds__(kBlock) norm_fwd_kernel(const NormArgs a) {
-  constexpr int kRows = kBlock / TPR;
-  __shared__ float red[16];
-  const int t = threadIdx.x % TPR;
-  const float inv = 1.0f / static_cast<float>(a.cols);
-  using P = Pack<T, V>;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR; r < a.rows;
-       r += static_cast<int64_t>(gridDim.x) * kRows) {
-    const T *x = static_cast<const T *>(a.x) + r * a.ldx;
-    float v[N * V], s = 0.0f;
+// How rows are spread over threads: element j of thread t's vector i sits in column
+// (i * TPR + t) * V + j; V = 1 where rows are not aligned.  A thread works through its elements in
+// units of PAIRS pairs: a vector, or two single elements, of which the second may lie beyond the row
+// (it reads as 0).
+template <class T_, int TPR_, int V_, int N_, int INPUTS>
+struct Lay {
+  using T = T_;
+  using P = Pack<T, V_>;
+  static constexpr int TPR = TPR_, V = V_, N = N_, kElems = N * V;
+  static constexpr int kUnits = V == 1 ? N / 2 : N, kPairs = V == 1 ? 1 : V / 2;
+  static constexpr int kThreads = TPR > kBlock ? TPR : kBlock, kRows = kThreads / TPR;
+  static constexpr int kRowBytes = TPR * kElems * static_cast<int>(sizeof(T));   // padded
+  static constexpr int kSlot = kRows * (kRowBytes + (V == 1 ? 48 : 0)) * INPUTS;
+  // the blocks of an SM (launch bounds below) share 160 KB of it for their rings; more rows ahead
+  // than four changed nothing
+  static constexpr int kPerSm = INPUTS == 1 ? (kThreads == kBlock ? (V == 1 ? 3 : 4) : 2) : (kThreads == kBlock ? 2 : 1);
+  static constexpr int kFit = 160 * 1024 / kPerSm / kSlot;
+  static constexpr int kDepth = kFit > 4 ? 4 : kFit < 1 ? 1 : kFit;
+  static constexpr int kBytes = kSlot * kDepth;
+  static constexpr int kParam = kRowBytes;                                       // gamma, or beta
+
+  // Starts the copies of row `row` (the TPR threads together); `at` is this input's part of a slot.
+  static __device__ __forceinline__ void fetch(uint32_t at, const T *row, int cols, int pitch, int t, int group) {
+    if constexpr (V > 1) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + t) * V;
-      if (c < a.cols) {
-        const P p = *reinterpret_cast<const P *>(x + c);
+      for (int i = 0; i < N; ++i) {
+        const int c = (i * TPR + t) * V;
+        if (c < cols) copy16(at + (i * kThreads + threadIdx.x) * 16, row + c);
+      }
+    } else {
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15);
+      const uintptr_t hi = reinterpret_cast<uintptr_t>(row + cols);
+      for (uintptr_t p = lo + t * 16; p < hi; p += TPR * 16)
+        copy16(at + group * pitch + static_cast<uint32_t>(p - lo), reinterpret_cast<const void *>(p));
+    }
+  }
+  static __device__ __forceinline__ int column(int unit, int t) {
+    return V == 1 ? 2 * unit * TPR + t : (unit * TPR + t) * V;
+  }
+  static __device__ __forceinline__ bool second(int unit, int t, int cols) {
+    return V > 1 || column(unit, t) + TPR < cols;
+  }
+  static __device__ __forceinline__ void split(const P &p, float2 (&o)[kPairs]) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          v[i * V + j] = to_f32(p.v[j]);
-          s += v[i * V + j];
+    for (int j = 0; j < kPairs; ++j) o[j] = make_float2(to_f32(p.v[2 * j]), to_f32(p.v[2 * j + 1]));
+  }
+  // A unit of the row in a slot, and of gamma or beta.
+  static __device__ __forceinline__ void get(const uint8_t *at, const T *row, int cols, int pitch, int t, int group,
+                                             int unit, float2 (&o)[kPairs]) {
+    if constexpr (V > 1) {
+      split(*reinterpret_cast<const P *>(at + (unit * kThreads + threadIdx.x) * 16), o);
+    } else {
+      const T *p = reinterpret_cast<const T *>(at + group * pitch + (reinterpret_cast<uintptr_t>(row) & 15));
+      at_columns(p, cols, t, unit, o);
+    }
+  }
+  static __device__ __forceinline__ void at_columns(const T *p, int cols, int t, int unit, float2 (&o)[kPairs]) {
+    const int c = column(unit, t);
+    if constexpr (V > 1)
+      split(*reinterpret_cast<const P *>(p + c), o);
+    else
+      o[0] = make_float2(to_f32(p[c]), second(unit, t, cols) ? to_f32(p[c + TPR]) : 0.0f);
+  }
+  static __device__ __forceinline__ void put(T *p, int cols, int t, int unit, const float2 (&o)[kPairs]) {
+    const int c = column(unit, t);
+    if constexpr (V > 1) {
+      P q;
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) q.v[2 * j] = from_f32<T>(o[j].x), q.v[2 * j + 1] = from_f32<T>(o[j].y);
+      *reinterpret_cast<P *>(p + c) = q;
+    } else {
+      p[c] = from_f32<T>(o[0].x);
+      if (second(unit, t, cols)) p[c + TPR] = from_f32<T>(o[0].y);
+    }
+  }
+  // gamma or beta into shared memory, `none` where there is none.
+  static __device__ __forceinline__ void param(T *to, const void *from, int cols, float none) {
+    for (int c = threadIdx.x; c < cols; c += kThreads)
+      to[c] = from ? static_cast<const T *>(from)[c] : from_f32<T>(none);
+  }
+};
+
+template <class L>
+__global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_fwd_kernel(const NormArgs a) {
+  using T = typename L::T;
+  constexpr int TPR = L::TPR, V = L::V, D = L::kDepth, U = L::kUnits, Q = L::kPairs;
+  extern __shared__ __align__(16) uint8_t ring[];   // [kDepth] rows, gamma, beta
+  __shared__ float red_all[L::kRows][2][32];
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, cols = static_cast<int>(a.cols);
+  float(*red)[32] = red_all[group];
+  const float inv = 1.0f / static_cast<float>(cols);
+  const uint32_t at = smem_u32(ring);
+  T *gamma = reinterpret_cast<T *>(ring + L::kBytes), *beta = reinterpret_cast<T *>(ring + L::kBytes + L::kParam);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * L::kRows;
+  int64_t r = static_cast<int64_t>(blockIdx.x) * L::kRows + group, ahead = r;
+  const T *x = static_cast<const T *>(a.x) + r * a.ldx, *xa = x;     // this row, the row to fetch
+  T *y = static_cast<T *>(a.y) + r * a.ldy;
+  const int64_t xstep = step * a.ldx, ystep = step * a.ldy;
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d, ahead += step, xa += xstep) {
+    if (ahead < a.rows) L::fetch(at + d * L::kSlot, xa, cols, a.pitch, t, group);
+    copy_commit();
+  }
+  L::param(gamma, a.gamma, cols, 1.0f);
+  L::param(beta, a.beta, cols, 0.0f);
+  __syncthreads();
+  int slot = 0, fill = D - 1;
+  for (; r < a.rows; r += step, ahead += step, x += xstep, xa += xstep, y += ystep) {
+    if (ahead < a.rows) L::fetch(at + fill * L::kSlot, xa, cols, a.pitch, t, group);
+    copy_commit();
+    copy_wait<D - 1>();
+    if constexpr (V == 1) row_sync<TPR>(group);
+    float2 v[U][Q], s = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (L::column(i, t) < cols) {
+        L::get(ring + slot * L::kSlot, x, cols, a.pitch, t, group, i, v[i]);
+#pragma unroll
+        for (int j = 0; j < Q; ++j) s = add2(s, v[i][j]);
+      }
+    const float mean = row_sum<TPR>(s.x + s.y, red[0], group) * inv;
+    float2 q = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (L::column(i, t) < cols) {
+        const float2 shift = make_float2(-mean, L::second(i, t, cols) ? -mean : 0.0f);
+#pragma unroll
+        for (int j = 0; j < Q; ++j) {
+          v[i][j] = add2(v[i][j], shift);
+          q = fma2(v[i][j], v[i][j], q);
         }
       }
-    }
-    const float mean = row_sum<TPR>(s, red) * inv;
-    float q = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if ((i * TPR + t) * V < a.cols)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float d = v[i * V + j] - mean;
-          q = fmaf(d, d, q);
-        }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(q, red) * inv + a.eps);
+    const float rstd = inv_sqrt(row_sum<TPR>(q.x + q.y, red[1], group) * inv + a.eps);
     if (t == 0) {
       if (a.mean) a.mean[r] = mean;
       if (a.rstd) a.rstd[r] = rstd;
     }
-    T *y = static_cast<T *>(a.y) + r * a.ldy;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + t) * V;
-      if (c < a.cols) {
-        P g, b, o;
-        if (a.gamma) g = *reinterpret_cast<const P *>(static_cast<const T *>(a.gamma) + c);
-        if (a.beta) b = *reinterpret_cast<const P *>(static_cast<const T *>(a.beta) + c);
+    for (int i = 0; i < U; ++i)
+      if (L::column(i, t) < cols) {
+        float2 g[Q], b[Q];
+        L::at_columns(gamma, cols, t, i, g);
+        L::at_columns(beta, cols, t, i, b);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float f = (v[i * V + j] - mean) * rstd;
-          if (a.gamma) f *= to_f32(g.v[j]);
-          if (a.beta) f += to_f32(b.v[j]);
-          o.v[j] = from_f32<T>(f);
-        }
-        *reinterpret_cast<P *>(y + c) = o;
+        for (int j = 0; j < Q; ++j) g[j] = fma2(mul2(v[i][j], both(rstd)), g[j], b[j]);
+        L::put(y, cols, t, i, g);
       }
-    }
+    // (the slot read above is filled again in the next turn, behind this turn's barriers)
+    if constexpr (V == 1 && TPR == 32) __syncwarp();
+    slot = slot + 1 == D ? 0 : slot + 1;
+    fill = fill + 1 == D ? 0 : fill + 1;
   }
 }
 
 // Rows wider than the registers hold: three passes over the row, which stays in L2.
 template <class T>
 __global__ void __launch_bounds__(kBlock) norm_fwd_wide_kernel(const NormArgs a) {
-  __shared__ float red[16];
+  __shared__ float red[2][32];
   const float inv = 1.0f / static_cast<float>(a.cols);
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T *x = static_cast<const T *>(a.x) + r * a.ldx;
     float s = 0.0f, q = 0.0f;
     for (int64_t c = threadIdx.x; c < a.cols; c += kBlock) s += to_f32(x[c]);
-    const float mean = row_sum<kBlock>(s, red) * inv;
+    const float mean = row_sum<kBlock>(s, red[0], 0) * inv;
     for (int64_t c = threadIdx.x; c < a.cols; c += kBlock) {
       const float d = to_f32(x[c]) - mean;
       q = fmaf(d, d, q);
     }
-    const float rstd = 1.0f / sqrtf(row_sum<kBlock>(q, red) * inv + a.eps);
+    const float rstd = inv_sqrt(row_sum<kBlock>(q, red[1], 0) * inv + a.eps);
     if (threadIdx.x == 0) {
       if (a.mean) a.mean[r] = mean;
       if (a.rstd) a.rstd[r] = rstd;
@@ -159,93 +314,140 @@ __global__ void __launch_bounds__(kBlock) norm_fwd_wide_kernel(const NormArgs a)
   }
 }
 
-template <class T, int TPR, int V, int N>
-__global__ void __launch_bounds__(kBlock) norm_bwd_kernel(const NormArgs a) {
-  constexpr int kRows = kBlock / TPR;
-  __shared__ float red[16];
-  extern __shared__ float acc[];          // TPR == 32: [2][cols], the block's column sums
-  const int t = threadIdx.x % TPR;
-  const float inv = 1.0f / static_cast<float>(a.cols);
-  using P = Pack<T, V>;
-  float dg[N * V], db[N * V];
+template <class L>
+__global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_bwd_kernel(const NormArgs a) {
+  using T = typename L::T;
+  constexpr int TPR = L::TPR, V = L::V, D = L::kDepth, U = L::kUnits, Q = L::kPairs;
+  // 32 elements a thread and their two sums fill the registers: those rows are read from their slot
+  // again for dx
+  constexpr bool kKeep = L::kElems <= 16;
+  extern __shared__ __align__(16) uint8_t ring[];   // [kDepth][x, dy], gamma; in the end [kRows][2][cols] sums
+  __shared__ float red_all[L::kRows][2][32];
+  let_next_start();
+  const int t = threadIdx.x % TPR, group = threadIdx.x / TPR, cols = static_cast<int>(a.cols);
+  float(*red)[32] = red_all[group];
+  const float inv = 1.0f / static_cast<float>(cols);
+  constexpr int kHalf = L::kSlot / 2;               // dy's part of a slot
+  const uint32_t at = smem_u32(ring);
+  T *gamma = reinterpret_cast<T *>(ring + L::kBytes);
+  float2 dg[U][Q], db[U][Q];
 #pragma unroll
-  for (int i = 0; i < N * V; ++i) dg[i] = db[i] = 0.0f;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR; r < a.rows;
-       r += static_cast<int64_t>(gridDim.x) * kRows) {
-    const T *x = static_cast<const T *>(a.x) + r * a.ldx;
-    const T *dy = static_cast<const T *>(a.dy) + r * a.lddy;
-    const float mean = a.mean[r], rstd = a.rstd[r];
-    float xh[N * V], g[N * V], s1 = 0.0f, s2 = 0.0f;
+  for (int i = 0; i < U; ++i)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + t) * V;
-      if (c < a.cols) {
-        const P px = *reinterpret_cast<const P *>(x + c);
-        const P pd = *reinterpret_cast<const P *>(dy + c);
-        P pg;
-        if (a.gamma) pg = *reinterpret_cast<const P *>(static_cast<const T *>(a.gamma) + c);
+    for (int j = 0; j < Q; ++j) dg[i][j] = db[i][j] = both(0.0f);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * L::kRows;
+  int64_t r = static_cast<int64_t>(blockIdx.x) * L::kRows + group, ahead = r;
+  const T *x = static_cast<const T *>(a.x) + r * a.ldx, *xa = x;      // this row, the row to fetch
+  const T *dy = static_cast<const T *>(a.dy) + r * a.lddy, *da = dy;
+  T *dx = static_cast<T *>(a.y) + r * a.ldy;
+  const int64_t xstep = step * a.ldx, dstep = step * a.lddy, ystep = step * a.ldy;
+  auto fetch = [&](int slot) {
+    L::fetch(at + slot * L::kSlot, xa, cols, a.pitch, t, group);
+    L::fetch(at + slot * L::kSlot + kHalf, da, cols, a.pitch, t, group);
+  };
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int k = i * V + j;
-          const float d = to_f32(pd.v[j]);
-          xh[k] = (to_f32(px.v[j]) - mean) * rstd;
-          g[k] = a.gamma ? d * to_f32(pg.v[j]) : d;
-          s1 += g[k];
-          s2 = fmaf(g[k], xh[k], s2);
-          dg[k] = fmaf(d, xh[k], dg[k]);
-          db[k] += d;
+  for (int d = 0; d < D - 1; ++d, ahead += step, xa += xstep, da += dstep) {
+    if (ahead < a.rows) fetch(d);
+    copy_commit();
+  }
+  L::param(gamma, a.gamma, cols, 1.0f);
+  __syncthreads();
+  int slot = 0, fill = D - 1;
+  float next_mean = r < a.rows ? a.mean[r] : 0.0f, next_rstd = r < a.rows ? a.rstd[r] : 0.0f;
+  for (int turn = 0; r < a.rows;
+       r += step, ahead += step, x += xstep, xa += xstep, dy += dstep, da += dstep, dx += ystep, turn ^= 1) {
+    if (ahead < a.rows) fetch(fill);
+    copy_commit();
+    const float mean = next_mean, rstd = next_rstd;
+    if (r + step < a.rows) next_mean = a.mean[r + step], next_rstd = a.rstd[r + step];
+    copy_wait<D - 1>();
+    if constexpr (V == 1) row_sync<TPR>(group);
+    const uint8_t *sx = ring + slot * L::kSlot, *sd = sx + kHalf;
+    const float2 shift = both(-mean), scale = both(rstd);
+    float2 xh[kKeep ? U : 1][Q], g[kKeep ? U : 1][Q], s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (L::column(i, t) < cols) {
+        float2 px[Q], pd[Q], pg[Q];
+        L::get(sx, x, cols, a.pitch, t, group, i, px);
+        L::get(sd, dy, cols, a.pitch, t, group, i, pd);
+        L::at_columns(gamma, cols, t, i, pg);
+#pragma unroll
+        for (int j = 0; j < Q; ++j) {
+          const float2 h = mul2(add2(px[j], shift), scale), e = mul2(pd[j], pg[j]);
+          s1 = add2(s1, e);
+          s2 = fma2(e, h, s2);
+          dg[i][j] = fma2(pd[j], h, dg[i][j]);
+          db[i][j] = add2(db[i][j], pd[j]);
+          if constexpr (kKeep) xh[i][j] = h, g[i][j] = e;
         }
       }
-    }
-    row_sum2<TPR>(s1, s2, red);
-    if (!a.y) continue;
-    s1 *= inv;
-    s2 *= inv;
-    T *dx = static_cast<T *>(a.y) + r * a.ldy;
+    float m1 = s1.x + s1.y, m2 = s2.x + s2.y;
+    row_sum2<TPR>(m1, m2, red[turn], group);
+    if (a.y) {
+      const float2 n1 = both(-m1 * inv), n2 = both(-m2 * inv);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + t) * V;
-      if (c < a.cols) {
-        P o;
+      for (int i = 0; i < U; ++i)
+        if (L::column(i, t) < cols) {
+          float2 px[Q], pd[Q], pg[Q];
+          if constexpr (!kKeep) {
+            L::get(sx, x, cols, a.pitch, t, group, i, px);
+            L::get(sd, dy, cols, a.pitch, t, group, i, pd);
+            L::at_columns(gamma, cols, t, i, pg);
+          }
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int k = i * V + j;
-          o.v[j] = from_f32<T>(rstd * (g[k] - s1 - xh[k] * s2));
+          for (int j = 0; j < Q; ++j) {
+            float2 h, e;
+            if constexpr (kKeep)
+              h = xh[i][j], e = g[i][j];
+            else
+              h = mul2(add2(px[j], shift), scale), e = mul2(pd[j], pg[j]);
+            px[j] = mul2(fma2(h, n2, add2(e, n1)), scale);
+          }
+          L::put(dx, cols, t, i, px);
         }
-        *reinterpret_cast<P *>(dx + c) = o;
-      }
     }
+    // the slot read above is filled again in the next turn
+    if constexpr (V == 1 && (TPR == 32 || !kKeep)) row_sync<TPR>(group);
+    slot = slot + 1 == D ? 0 : slot + 1;
+    fill = fill + 1 == D ? 0 : fill + 1;
   }
   if (!a.part) return;
   float *part = a.part + 2 * a.cols * blockIdx.x;
-  if constexpr (TPR == 32) {
-    // the block's warps add their sums one after another (a fixed order)
-    for (int w = 0; w < kRows; ++w) {
-      if (static_cast<int>(threadIdx.x >> 5) == w) {
+  auto give = [&](float *to) {   // this row's sums, [2][cols]
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int c = (i * TPR + t) * V;
-          if (c < a.cols)
+    for (int i = 0; i < U; ++i) {
+      const int c = L::column(i, t);
+      if (c < cols) {
+        if constexpr (V == 1) {
+          to[c] = dg[i][0].x;
+          to[cols + c] = db[i][0].x;
+          if (L::second(i, t, cols)) to[c + TPR] = dg[i][0].y, to[cols + c + TPR] = db[i][0].y;
+        } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              acc[c + j] = (w ? acc[c + j] : 0.0f) + dg[i * V + j];
-              acc[a.cols + c + j] = (w ? acc[a.cols + c + j] : 0.0f) + db[i * V + j];
-            }
+          for (int j = 0; j < Q; j += 2) {
+            *reinterpret_cast<float4 *>(to + c + 2 * j) = make_float4(dg[i][j].x, dg[i][j].y, dg[i][j + 1].x, dg[i][j + 1].y);
+            *reinterpret_cast<float4 *>(to + cols + c + 2 * j) =
+                make_float4(db[i][j].x, db[i][j].y, db[i][j + 1].x, db[i][j + 1].y);
+          }
         }
       }
-      __syncthreads();
     }
-    for (int c = threadIdx.x; c < 2 * a.cols; c += kBlock) part[c] = acc[c];
-  } else {
+  };
+  if constexpr (L::kRows == 1) {
+    give(part);
+  } else {   // the block's rows meet in the ring, whose copies have all been used, and are added in order
+    static_assert(L::kBytes >= L::kRows * 2 * TPR * L::kElems * 4, "the sums need the ring's room");
+    float *acc = reinterpret_cast<float *>(ring);
+    copy_wait<0>();
+    __syncthreads();
+    give(acc + group * 2 * cols);
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * cols; c += L::kThreads) {
+      float v = acc[c];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = (i * TPR + t) * V;
-      if (c < a.cols)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          part[c + j] = dg[i * V + j];
-          part[a.cols + c + j] = db[i * V + j];
-        }
+      for (int w = 1; w < L::kRows; ++w) v += acc[w * 2 * cols + c];
+      part[c] = v;
     }
   }
 }
@@ -253,7 +455,8 @@ __global__ void __launch_bounds__(kBlock) norm_bwd_kernel(const NormArgs a) {
 // Wide rows: dx row by row, the column sums by a block per 32 columns (norm_cols_wide_kernel).
 template <class T>
 __global__ void __launch_bounds__(kBlock) norm_bwd_wide_kernel(const NormArgs a) {
-  __shared__ float red[16];
+  __shared__ float red[2][32];
+  int turn = 0;
   const float inv = 1.0f / static_cast<float>(a.cols);
   const T *gamma = static_cast<const T *>(a.gamma);
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -266,7 +469,8 @@ __global__ void __launch_bounds__(kBlock) norm_bwd_wide_kernel(const NormArgs a)
       s1 += g;
       s2 = fmaf(g, (to_f32(x[c]) - mean) * rstd, s2);
     }
-    row_sum2<kBlock>(s1, s2, red);
+    row_sum2<kBlock>(s1, s2, red[turn], 0);
+    turn ^= 1;
     s1 *= inv;
     s2 *= inv;
     T *dx = static_cast<T *>(a.y) + r * a.ldy;
@@ -306,25 +510,49 @@ __global__ void __launch_bounds__(kBlock) norm_cols_wide_kernel(const NormArgs a
   }
 }
 
-// [parts][n] -> out[n]: 32 columns x 8 lanes of parts per block, added in a fixed order.
-template <class T>
-__global__ void __launch_bounds__(kBlock)
+// [parts][n] -> out[n] (and out2 from out_n on): 32 columns x LANES per block; a lane adds every
+// LANES-th partial in order, then the lanes are added in order.
+template <class T, int LANES>
+__global__ void __launch_bounds__(32 * LANES)
     reduce_columns_kernel(const float *__restrict__ part, int parts, int64_t n, T *__restrict__ out,
                           int64_t out_n, T *__restrict__ out2) {
-  __shared__ float s[8][33];
+  __shared__ float s[LANES][33];
+  wait_for_previous();
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
   const int lane = threadIdx.x >> 5;
   float v = 0.0f;
   if (c < n)
-    for (int p = lane; p < parts; p += 8) v += part[p * n + c];
+#pragma unroll 8
+    for (int p = lane; p < parts; p += LANES) v += part[p * n + c];
   s[lane][threadIdx.x & 31] = v;
   __syncthreads();
   if (threadIdx.x < 32 && c < n) {
     v = 0.0f;
-    for (int i = 0; i < 8; ++i) v += s[i][threadIdx.x];
-    T *o = c < out_n ? out + c : (out2 ? out2 + (c - out_n) : nullptr);
-    if (o && (c >= out_n || out)) *o = from_f32<T>(v);
+#pragma unroll
+    for (int i = 0; i < LANES; ++i) v += s[i][threadIdx.x];
+    if (c < out_n) {
+      if (out) out[c] = from_f32<T>(v);
+    } else if (out2) {
+      out2[c - out_n] = from_f32<T>(v);
+    }
   }
+}
+
+// Launched so that it may start while the kernel that writes the partials still runs.
+template <class T, int LANES>
+int launch_reduce(const float *part, int parts, int64_t n, T *out, int64_t out_n, T *out2, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((n + 31) / 32));
+  cfg.blockDim = dim3(32 * LANES);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  PTB_CUDA(cudaLaunchKernelEx(&cfg, reduce_columns_kernel<T, LANES>, part, parts, n, out, out_n, out2));
+  count_launch();
+  return 0;
 }
 
 int64_t grid_rows(const pt_b200_ops *h, int64_t rows, int rows_per_block, int per_sm) {
@@ -333,56 +561,75 @@ int64_t grid_rows(const pt_b200_ops *h, int64_t rows, int rows_per_block, int pe
   return want < cap ? want : cap;
 }
 
-// Backward blocks: at most this many rows of partials.
-constexpr int kBwdPerSm = 4;
+// fn.template operator()<TPR, V, N>() for the threads and elements of a row.  Few elements a thread
+// where there are too few rows to fill the GPU (`few`), where one row's latency counts: 64 x 4096 fp32
+// backward took 10.3 us with 32 elements and 7.7 with 16.  Backward, rows of up to 2048 keep 8 or 16
+// elements, whose sums leave room for more rows at once (8192 x 1000 fp16 16 us, with 32 elements 32).
+template <class T, bool VEC, bool FORWARD, class F>
+int pick(int64_t cols, bool few, F &&fn) {
+  constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  if (cols <= 256) return fn.template operator()<32, V, 8 / V>();
+  if (cols <= 512) return fn.template operator()<32, V, 16 / V>();
+  if (cols <= 1024 && (few || !FORWARD)) return fn.template operator()<128, V, 8 / V>();
+  if (cols <= 4096 && few) return fn.template operator()<512, V, 8 / V>();
+  if (cols <= 8192 && (few || !FORWARD) && cols > 4096) return fn.template operator()<512, V, 16 / V>();
+  if constexpr (FORWARD) {
+    if (cols <= 1024) return fn.template operator()<32, V, 32 / V>();
+    if (cols <= 2048) return fn.template operator()<64, V, 32 / V>();
+    if (cols <= 8192 && cols > 4096) return fn.template operator()<256, V, 32 / V>();
+  } else {
+    if (cols <= 2048) return fn.template operator()<128, V, 16 / V>();
+  }
+  if (cols <= 4096) return fn.template operator()<128, V, 32 / V>();
+  return fn.template operator()<512, V, 32 / V>();
+}
+bool few_rows(const pt_b200_ops *h, int64_t rows) { return rows < 4 * h->sms; }
+
+// Backward blocks, which is the number of rows of partials: as many as run at once (two of 256
+// threads on an SM, one of 512).
 int bwd_blocks(const pt_b200_ops *h, int64_t rows, int64_t cols) {
   if (cols > kMaxRegCols) return static_cast<int>(rows < 8 * 64 ? (rows + 7) / 8 : 64);
-  return static_cast<int>(grid_rows(h, rows, cols <= 1024 ? kBlock / 32 : 1, kBwdPerSm));
-}
-
-// fn.template operator()<TPR, V, N>() for the smallest instance that holds `cols`.
-template <class T, bool VEC, class F>
-int pick(int64_t cols, F &&fn) {
-  constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
-  if (cols <= 1024) {
-    const int64_t n = (cols + 32 * V - 1) / (32 * V);
-    if (n * V <= 8) return fn.template operator()<32, V, 8 / V>();
-    if (n * V <= 16) return fn.template operator()<32, V, 16 / V>();
-    return fn.template operator()<32, V, 32 / V>();
-  }
-  const int64_t n = (cols + 256 * V - 1) / (256 * V);
-  if (n * V <= 8) return fn.template operator()<256, V, 8 / V>();
-  if (n * V <= 16) return fn.template operator()<256, V, 16 / V>();
-  if (n * V <= 32) return fn.template operator()<256, V, 32 / V>();
-  return fn.template operator()<256, V, 64 / V>();
+  const bool few = few_rows(h, rows);
+  const int per_block = cols <= 512 ? 8 : cols <= 1024 || (cols <= 4096 && !few) ? 2 : 1;
+  return static_cast<int>(grid_rows(h, rows, per_block, cols <= 1024 || (cols <= 4096 && !few) ? 2 : 1));
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <class T, bool VEC>
+// Shared memory beyond 48 KB has to be allowed once per kernel and device; it is set at every launch
+// that needs it, which costs nothing next to the launch.
+template <class K>
+int launch_rows(K kernel, int64_t blocks, int threads, size_t smem, const NormArgs &a, cudaStream_t st) {
+  if (smem > 40 * 1024)   // (beside the static part, within the 48 KB that need no permission)
+    PTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+  kernel<<<static_cast<unsigned>(blocks), threads, smem, st>>>(a);
+  PTB_CUDA(cudaGetLastError());
+  count_launch();
+  return 0;
+}
+
+template <class T>
 struct FwdLaunch {
   const pt_b200_ops *h;
   const NormArgs &a;
   cudaStream_t st;
   template <int TPR, int V, int N>
   int operator()() const {
-    norm_fwd_kernel<T, TPR, V, N>
-        <<<static_cast<unsigned>(grid_rows(h, a.rows, kBlock / TPR, 8)), kBlock, 0, st>>>(a);
-    return 0;
+    using L = Lay<T, TPR, V, N, 1>;
+    return launch_rows(norm_fwd_kernel<L>, grid_rows(h, a.rows, L::kRows, L::kPerSm), L::kThreads,
+                       L::kBytes + 2 * L::kParam, a, st);
   }
 };
 
-template <class T, bool VEC>
+template <class T>
 struct BwdLaunch {
   const pt_b200_ops *h;
   const NormArgs &a;
   cudaStream_t st;
   template <int TPR, int V, int N>
   int operator()() const {
-    const size_t smem = TPR == 32 && a.part ? static_cast<size_t>(2 * a.cols) * 4 : 0;
-    norm_bwd_kernel<T, TPR, V, N>
-        <<<static_cast<unsigned>(bwd_blocks(h, a.rows, a.cols)), kBlock, smem, st>>>(a);
-    return 0;
+    using L = Lay<T, TPR, V, N, 2>;
+    return launch_rows(norm_bwd_kernel<L>, bwd_blocks(h, a.rows, a.cols), L::kThreads, L::kBytes + L::kParam, a, st);
   }
 };
 
@@ -391,11 +638,7 @@ struct BwdLaunch {
 namespace ptb {
 template <class T>
 int reduce_columns(const float *part, int parts, int64_t n, T *out, cudaStream_t st) {
-  reduce_columns_kernel<T><<<static_cast<unsigned>((n + 31) / 32), kBlock, 0, st>>>(part, parts, n, out,
-                                                                                   n, nullptr);
-  PTB_CUDA(cudaGetLastError());
-  count_launch();
-  return 0;
+  return launch_reduce<T, 8>(part, parts, n, out, n, nullptr, st);
 }
 template int reduce_columns<float>(const float *, int, int64_t, float *, cudaStream_t);
 template int reduce_columns<__nv_bfloat16>(const float *, int, int64_t, __nv_bfloat16 *, cudaStream_t);
@@ -406,7 +649,8 @@ extern "C" int pt_b200_layer_norm(pt_b200_ops *h, void *stream, const pt_b200_no
   PTB_REQUIRE(h && p, "pt_b200_layer_norm: NULL handle or arguments");
   PTB_REQUIRE(p->dtype >= PT_B200_F32 && p->dtype <= PT_B200_F16, "pt_b200_layer_norm: unknown element type %d",
               p->dtype);
-  PTB_REQUIRE(p->rows >= 0 && p->cols > 0 && p->cols <= (int64_t(1) << 30), "pt_b200_layer_norm: rows %lld x cols %lld",
+  PTB_REQUIRE(p->rows >= 0 && p->rows < (int64_t(1) << 31) && p->cols > 0 && p->cols <= (int64_t(1) << 30),
+              "pt_b200_layer_norm: rows %lld x cols %lld",
               (long long)p->rows, (long long)p->cols);
   const int eb = dtype_bytes(p->dtype);
   PTB_REQUIRE(rows_ok(p->x, p->rows, p->cols, p->ldx, eb) && rows_ok(p->y, p->rows, p->cols, p->ldy, eb),
@@ -428,22 +672,18 @@ extern "C" int pt_b200_layer_norm(pt_b200_ops *h, void *stream, const pt_b200_no
   a.ldx = p->ldx;
   a.ldy = p->ldy;
   a.eps = p->eps;
+  a.pitch = static_cast<int>(round_up(p->cols * eb, 16) + 32);
   const int v = 16 / eb;
   const bool vec = p->cols % v == 0 && (p->rows == 1 || (p->ldx % v == 0 && p->ldy % v == 0)) &&
                    aligned16(p->x) && aligned16(p->y) && aligned16(p->gamma) && aligned16(p->beta);
-  const int rc = with_dtype(p->dtype, [&](auto *z) {
+  return with_dtype(p->dtype, [&](auto *z) -> int {
     using T = std::remove_pointer_t<decltype(z)>;
-    if (a.cols > kMaxRegCols) {
-      norm_fwd_wide_kernel<T><<<static_cast<unsigned>(grid_rows(h, a.rows, 1, 8)), kBlock, 0, st>>>(a);
-      return 0;
-    }
-    return vec ? pick<T, true>(a.cols, FwdLaunch<T, true>{h, a, st})
-               : pick<T, false>(a.cols, FwdLaunch<T, false>{h, a, st});
+    if (a.cols > kMaxRegCols)
+      return launch_rows(norm_fwd_wide_kernel<T>, grid_rows(h, a.rows, 1, 8), kBlock, 0, a, st);
+    const bool few = few_rows(h, a.rows);
+    return vec ? pick<T, true, true>(a.cols, few, FwdLaunch<T>{h, a, st})
+               : pick<T, false, true>(a.cols, few, FwdLaunch<T>{h, a, st});
   });
-  if (rc) return rc;
-  PTB_CUDA(cudaGetLastError());
-  count_launch();
-  return 0;
 }
 
 extern "C" int64_t pt_b200_layer_norm_backward_work(const pt_b200_ops *h, int64_t rows, int64_t cols) {
@@ -456,7 +696,7 @@ extern "C" int pt_b200_layer_norm_backward(pt_b200_ops *h, void *stream,
   PTB_REQUIRE(h && p, "pt_b200_layer_norm_backward: NULL handle or arguments");
   PTB_REQUIRE(p->dtype >= PT_B200_F32 && p->dtype <= PT_B200_F16,
               "pt_b200_layer_norm_backward: unknown element type %d", p->dtype);
-  PTB_REQUIRE(p->rows >= 0 && p->cols > 0 && p->cols <= (int64_t(1) << 30),
+  PTB_REQUIRE(p->rows >= 0 && p->rows < (int64_t(1) << 31) && p->cols > 0 && p->cols <= (int64_t(1) << 30),
               "pt_b200_layer_norm_backward: rows %lld x cols %lld", (long long)p->rows, (long long)p->cols);
   const int eb = dtype_bytes(p->dtype);
   PTB_REQUIRE(rows_ok(p->x, p->rows, p->cols, p->ldx, eb) && rows_ok(p->dy, p->rows, p->cols, p->lddy, eb) &&
@@ -490,6 +730,7 @@ extern "C" int pt_b200_layer_norm_backward(pt_b200_ops *h, void *stream,
   a.ldx = p->ldx;
   a.lddy = p->lddy;
   a.ldy = p->lddx;
+  a.pitch = static_cast<int>(round_up(p->cols * eb, 16) + 32);
   const int v = 16 / eb;
   const bool vec = p->cols % v == 0 &&
                    (p->rows == 1 || (p->ldx % v == 0 && p->lddy % v == 0 && (!p->dx || p->lddx % v == 0))) &&
@@ -498,29 +739,19 @@ extern "C" int pt_b200_layer_norm_backward(pt_b200_ops *h, void *stream,
     using T = std::remove_pointer_t<decltype(z)>;
     int parts = bwd_blocks(h, a.rows, a.cols);
     if (a.cols > kMaxRegCols) {
-      if (a.y) {
-        norm_bwd_wide_kernel<T><<<static_cast<unsigned>(grid_rows(h, a.rows, 1, 8)), kBlock, 0, st>>>(a);
-        PTB_CUDA(cudaGetLastError());
-        count_launch();
-      }
+      if (a.y && launch_rows(norm_bwd_wide_kernel<T>, grid_rows(h, a.rows, 1, 8), kBlock, 0, a, st)) return -1;
       if (sums) {
         norm_cols_wide_kernel<T>
             <<<dim3(static_cast<unsigned>((a.cols + 31) / 32), parts), kBlock, 0, st>>>(a);
         PTB_CUDA(cudaGetLastError());
         count_launch();
       }
-    } else {
-      if (vec ? pick<T, true>(a.cols, BwdLaunch<T, true>{h, a, st})
-              : pick<T, false>(a.cols, BwdLaunch<T, false>{h, a, st}))
-        return -1;
-      PTB_CUDA(cudaGetLastError());
-      count_launch();
+    } else if (vec ? pick<T, true, false>(a.cols, few_rows(h, a.rows), BwdLaunch<T>{h, a, st})
+                   : pick<T, false, false>(a.cols, few_rows(h, a.rows), BwdLaunch<T>{h, a, st})) {
+      return -1;
     }
     if (!sums) return 0;
-    reduce_columns_kernel<T><<<static_cast<unsigned>((2 * a.cols + 31) / 32), kBlock, 0, st>>>(
-        a.part, parts, 2 * a.cols, static_cast<T *>(p->dgamma), a.cols, static_cast<T *>(p->dbeta));
-    PTB_CUDA(cudaGetLastError());
-    count_launch();
-    return 0;
+    return launch_reduce<T, 32>(a.part, parts, 2 * a.cols, static_cast<T *>(p->dgamma), a.cols,
+                                static_cast<T *>(p->dbeta), st);
   });
 }

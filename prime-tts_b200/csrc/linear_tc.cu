@@ -569,6 +569,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // ------------------------------------------------------------------------------ operand passes
 constexpr int kPrepBlock = 256;
 constexpr int kPrepRows = 2;   // rows a thread has in flight
+constexpr int kPrepPerSm = 3;  // blocks of a pass that run on one SM at once, and that it is cut into
 
 template <class T>
 struct Eight {
@@ -650,7 +651,7 @@ struct PrepRows {
 // Bound by HBM: src and pre are read once and dst is written once, 16 bytes a thread at a time
 // where rows are aligned.
 template <class T>
-__global__ void __launch_bounds__(kPrepBlock, 3) prep_kernel(const __grid_constant__ PrepJobs jobs) {
+__global__ void __launch_bounds__(kPrepBlock, kPrepPerSm) prep_kernel(const __grid_constant__ PrepJobs jobs) {
   __shared__ float red[kPrepBlock * 8];
   let_next_start();
   int job = 0, block = blockIdx.x;
@@ -852,7 +853,7 @@ int tc_row_blocks(const pt_b200_ops *h, int64_t rows, int64_t cols) {
   const int lanes = prep_lanes(cols), height = kPrepBlock / lanes;
   const int64_t col_blocks = (cols + lanes * 8 - 1) / (lanes * 8);
   const int64_t want = (rows + height * kPrepRows - 1) / (height * kPrepRows);
-  const int64_t cap = std::max<int64_t>(1, static_cast<int64_t>(h->sms) * 4 / col_blocks);
+  const int64_t cap = std::max<int64_t>(1, static_cast<int64_t>(h->sms) * kPrepPerSm / col_blocks);
   return static_cast<int>(std::min(want, cap));
 }
 

@@ -24,7 +24,7 @@ struct TcProduct {
 // would round up to infinity is truncated there instead.
 __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&o)[3]) {
   o[0] = __float2bfloat16_rn(x);
-  if (!isfinite(__bfloat162float(o[0]))) {
+  if (!(fabsf(x) <= 3.38953139e38f)) {   // beyond the largest finite bf16, or NaN
     if (!isfinite(x)) {
       o[1] = o[2] = __float2bfloat16_rn(0.0f);
       return;

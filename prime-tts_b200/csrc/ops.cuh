@@ -73,19 +73,31 @@ inline int dtype_bytes(int dtype) { return dtype == PT_B200_F32 ? 4 : 2; }
 // The normal distribution function is 1 - h(p) / 2 for p >= 0 and h(-p) / 2 below, where h(p) =
 // erfc(p / sqrt 2) = poly(t) exp(-p^2 / 2), t = 1 / (1 + 0.3275911 p / sqrt 2): Abramowitz and
 // Stegun, Handbook of Mathematical Functions, 7.1.26, off by at most 1.5e-7 / 2.  The exponential
-// is also the density's, so value and slope of gelu cost one exponential and one reciprocal; erff
-// took 1.3 times as long in the 16384 x 4096 bf16 gradient pass.
+// is also the density's, so value and slope of gelu cost one exponential and one reciprocal.
 constexpr float kSqrtHalf = 0.70710678118654752f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
+// The hardware's 2^x and 1 / x (errors of about 2^-22), denormal results as zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+
 __device__ __forceinline__ void normal_cdf(float p, float *cdf, float *gauss) {
-  const float e = __expf(-0.5f * p * p);
-  const float t = __fdividef(1.0f, fmaf(0.3275911f * kSqrtHalf, fabsf(p), 1.0f));
-  float q = fmaf(1.061405429f, t, -1.453152027f);
-  q = fmaf(q, t, 1.421413741f);
-  q = fmaf(q, t, -0.284496736f);
-  q = fmaf(q, t, 0.254829592f);
-  const float h = 0.5f * q * t * e;
+  const float e = exp2_fast(p * p * (-0.5f * kLog2E));
+  const float t = rcp_fast(fmaf(0.3275911f * kSqrtHalf, fabsf(p), 1.0f));
+  float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);   // (half the polynomial)
+  q = fmaf(q, t, 0.5f * 1.421413741f);
+  q = fmaf(q, t, 0.5f * -0.284496736f);
+  q = fmaf(q, t, 0.5f * 0.254829592f);
+  const float h = q * t * e;
   *cdf = p < 0.0f ? h : 1.0f - h;
   *gauss = e;
 }
@@ -99,7 +111,7 @@ __device__ __forceinline__ float act_value(float p, float slope) {
     normal_cdf(p, &cdf, &gauss);
     return p * cdf;
   }
-  if constexpr (ACT == PT_B200_ACT_SILU) return __fdividef(p, 1.0f + __expf(-p));
+  if constexpr (ACT == PT_B200_ACT_SILU) return p * rcp_fast(1.0f + exp2_fast(p * -kLog2E));
   return p;
 }
 
@@ -113,7 +125,7 @@ __device__ __forceinline__ float act_grad(float p, float slope) {
     return fmaf(p * kInvSqrt2Pi, gauss, cdf);
   }
   if constexpr (ACT == PT_B200_ACT_SILU) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-p));
+    const float s = rcp_fast(1.0f + exp2_fast(p * -kLog2E));
     return s * (1.0f + p * (1.0f - s));
   }
   return 1.0f;
