@@ -4,11 +4,130 @@
 //   dpre = dy * act'(pre);  dx = dpre W;  dW = dpre^T x;  db = sum over rows of dpre
 //
 // The three products run on the tensor cores (linear_tc.cu).
+#include <type_traits>
+
 #include "linear_tc.cuh"
 
 using namespace ptb;
 
 namespace {
+
+struct FewArgs {
+  const void *x, *w;
+  int64_t in, out, ldx, ldw;
+  int rows, shares;     // shares: warps that split a channel's k
+  LinearEpi e;
+};
+
+// ---- a few rows (single tokens): every weight is read once and used for all of them, so the call is
+// bound by the weights' bytes, and by its latency where they are few.  A warp takes two channels and a
+// share of k: it reads 16 bytes of each weight row and of each row of x (which stays in L1) per lane
+// and step, kAhead steps in flight with no branch between the loads, and adds up in fp32 FMAs.
+// Lanes, then the warps that share a channel's k, add up in a fixed order.  Measured against the
+// tensor cores (tc): bf16, 4096 to 1024, 4 rows 5.6 us (tc 6.8), 8 rows 7.5 (6.8); 4096 to 4096, 2
+// rows 8.0 (8.7), 4 rows 11.1 (8.7); fp32, which the tensor cores need in planes first, 4096 to 4096,
+// 8 rows 17.4 (48).
+constexpr int kFewGroup = 8, kFewWarps = 8, kFewChans = 2, kFewFill = 16;
+
+// Sums of v[0 .. N) over the warp, by halves: N / 2 + N / 4 + ... exchanges, not 5 N.  Lane l holds
+// the sum of value (l / (32 / N)).
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N], int lane) {
+  int o = 16;
+#pragma unroll
+  for (int n = N; n > 1; n /= 2, o /= 2) {
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const bool up = lane & o;
+      const float give = up ? v[i] : v[i + n / 2], keep = up ? v[i + n / 2] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  for (; o; o /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
+
+template <class T, int R, bool VEC>
+__global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const FewArgs a) {
+  constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1, kAhead = VEC ? (R <= 2 ? 4 : R == 4 ? 2 : 1) : 4;
+  constexpr int kSums = kFewChans * R;
+  using P = Pack<T, V>;
+  __shared__ float part[kFewWarps][kSums];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int share = warp % a.shares, team = warp / a.shares;
+  const int row0 = blockIdx.y * kFewGroup, rows = min(a.rows - row0, kFewGroup);
+  const int64_t chan = (static_cast<int64_t>(blockIdx.x) * (kFewWarps / a.shares) + team) * kFewChans;
+  float acc[kSums];
+#pragma unroll
+  for (int i = 0; i < kSums; ++i) acc[i] = 0.0f;
+  if (chan < a.out) {
+    const int64_t step = static_cast<int64_t>(a.shares) * 32 * V;
+    int64_t k = (share * 32 + lane) * V;
+    const T *w[kFewChans], *x[R];
+    w[0] = static_cast<const T *>(a.w) + chan * a.ldw + k;
+    w[1] = w[0] + (chan + 1 < a.out ? a.ldw : 0);          // (a last single channel twice)
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r] = static_cast<const T *>(a.x) + (row0 + (r < rows ? r : 0)) * a.ldx + k;
+    auto steps = [&](auto count) {
+      constexpr int A = decltype(count)::value;
+      P p[A][kFewChans], q[A][R];
+#pragma unroll
+      for (int u = 0; u < A; ++u) {
+#pragma unroll
+        for (int c = 0; c < kFewChans; ++c) p[u][c] = *reinterpret_cast<const P *>(w[c] + u * step);
+#pragma unroll
+        for (int r = 0; r < R; ++r) q[u][r] = *reinterpret_cast<const P *>(x[r] + u * step);
+      }
+#pragma unroll
+      for (int u = 0; u < A; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < kFewChans; ++c)
+              acc[c * R + r] = fmaf(to_f32(p[u][c].v[j]), to_f32(q[u][r].v[j]), acc[c * R + r]);
+#pragma unroll
+      for (int c = 0; c < kFewChans; ++c) w[c] += A * step;
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r] += A * step;
+      k += A * step;
+    };
+    while (k + (kAhead - 1) * step < a.in) steps(std::integral_constant<int, kAhead>{});
+    while (k < a.in) steps(std::integral_constant<int, 1>{});
+  }
+  __syncwarp();
+  const float v = warp_sums(acc, lane);
+  if (lane % (32 / kSums) == 0) part[warp][lane / (32 / kSums)] = v;
+  __syncthreads();
+  if (share == 0 && lane < kSums) {
+    const int c = lane / R, r = lane % R;
+    if (chan + c < a.out && r < rows) {
+      float t = 0.0f;
+      for (int s = 0; s < a.shares; ++s) t += part[warp + s][lane];
+      linear_store<T>(a.e, row0 + r, chan + c, t);
+    }
+  }
+}
+
+template <class T, bool VEC>
+int launch_few(const pt_b200_ops *h, const FewArgs &args, cudaStream_t st) {
+  constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  FewArgs a = args;
+  // share a channel's k among warps until there are kFewFill on every SM, or a share is a single step
+  const int64_t teams = (a.out + kFewChans - 1) / kFewChans;
+  a.shares = 1;
+  while (a.shares < kFewWarps && teams * a.shares < kFewFill * h->sms && a.in > a.shares * 32 * V) a.shares *= 2;
+  const int64_t per_block = kFewWarps / a.shares;
+  const unsigned blocks = static_cast<unsigned>((teams + per_block - 1) / per_block);
+  auto *kernel = a.rows == 1 ? linear_few_kernel<T, 1, VEC>
+                 : a.rows == 2 ? linear_few_kernel<T, 2, VEC>
+                 : a.rows <= 4 ? linear_few_kernel<T, 4, VEC> : linear_few_kernel<T, 8, VEC>;
+  kernel<<<dim3(blocks, (a.rows + kFewGroup - 1) / kFewGroup), kFewWarps * 32, 0, st>>>(a);
+  PTB_CUDA(cudaGetLastError());
+  count_launch();
+  return 0;
+}
 
 // An operand: the tensor itself where the tensor cores can read it, else its planes in the
 // workspace, which a pass of `jobs` fills.
@@ -37,10 +156,20 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
          n_out < (int64_t(1) << 30);
 }
 
+// Whether a call takes the few-rows kernel: while its FMAs cost less than what the tensor cores need
+// beside their products (a start, and planes where the operands cannot be read where they lie).
+bool few_rows(const pt_b200_linear_args *p) {
+  if (p->dtype == PT_B200_F32) return p->rows <= 2 * kFewGroup;
+  const bool direct = tc_direct(p->dtype, p->x, p->rows, p->ldx) && tc_direct(p->dtype, p->w, p->out, p->ldw);
+  if (!direct) return p->rows <= kFewGroup / 2 || (p->rows <= kFewGroup && p->in * p->out <= (1 << 22));
+  return p->rows <= 2 || (p->rows <= 4 && p->in * p->out <= (1 << 22));
+}
+
 }  // namespace
 
 extern "C" int64_t pt_b200_linear_work(const pt_b200_ops *h, const pt_b200_linear_args *p) {
   if (!h || !p || !sizes_ok(p->rows, p->in, p->out) || p->rows == 0) return 0;
+  if (few_rows(p)) return 0;
   return operand_bytes(p->dtype, p->x, p->rows, p->in, p->ldx) +
          operand_bytes(p->dtype, p->w, p->out, p->in, p->ldw);
 }
@@ -64,6 +193,19 @@ extern "C" int pt_b200_linear(pt_b200_ops *h, void *stream, const pt_b200_linear
   DeviceScope on(h->device);
   PTB_REQUIRE(on.ok, "pt_b200_linear: device %d cannot be used", h->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const LinearEpi epi{p->bias, p->residual, p->y, p->pre, p->ldr, p->ldy, p->ldp, p->act, p->slope};
+  if (few_rows(p)) {
+    const FewArgs a{p->x, p->w, p->in, p->out, p->ldx, p->ldw, static_cast<int>(p->rows), 1, epi};
+    const int v = 16 / eb;
+    auto aligned = [&](const void *q, int64_t rows, int64_t ld) {
+      return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows == 1 || ld % v == 0);
+    };
+    const bool vec = p->in % v == 0 && aligned(p->x, p->rows, p->ldx) && aligned(p->w, p->out, p->ldw);
+    return with_dtype(p->dtype, [&](auto *z) -> int {
+      using T = std::remove_pointer_t<decltype(z)>;
+      return vec ? launch_few<T, true>(h, a, st) : launch_few<T, false>(h, a, st);
+    });
+  }
   const int64_t need = pt_b200_linear_work(h, p);
   PTB_REQUIRE(need == 0 || (p->work && p->work_bytes >= need && reinterpret_cast<uintptr_t>(p->work) % 256 == 0),
               "pt_b200_linear: %lld bytes of 256-byte aligned workspace are needed, %lld given", (long long)need,
@@ -77,7 +219,7 @@ extern "C" int pt_b200_linear(pt_b200_ops *h, void *stream, const pt_b200_linear
   q.rows = p->rows;
   q.chans = p->out;
   q.k = p->in;
-  q.e = LinearEpi{p->bias, p->residual, p->y, p->pre, p->ldr, p->ldy, p->ldp, p->act, p->slope};
+  q.e = epi;
   if (tc_prep(p->dtype, jobs, n, st)) return -1;
   return tc_product(h, p->dtype, q, ColumnSums{}, n > 0, false, st);
 }

@@ -812,6 +812,10 @@ class Operators:
         self.h = h
         self.device = device
         self._types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+        # torch's current stream as a handle; its Stream object costs a microsecond to make
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self._stream = (lambda: raw(device)) if raw else (
+            lambda: torch.cuda.current_stream(device).cuda_stream)
 
     def close(self) -> None:
         if self.h:
@@ -828,9 +832,6 @@ class Operators:
         """Wait for torch's current stream and report device errors."""
         _check(self._lib.pt_b200_ops_sync(self.h, self._stream()), "pt_b200_ops_sync")
 
-    def _stream(self) -> int:
-        return self._torch.cuda.current_stream(self.device).cuda_stream
-
     def _type(self, t, what: str) -> int:
         """The element type of a call's first tensor."""
         code = self._types.get(t.dtype)
@@ -842,17 +843,19 @@ class Operators:
     def _rows(self, t, name: str, dtype, rows: int, cols: int):
         """(address, row stride) of a [..., cols] tensor seen as [rows][cols]."""
         shape = t.shape
-        if t.dtype != dtype or t.get_device() != self.device or len(shape) < 1 or shape[-1] != cols \
+        if t.dtype != dtype or t.get_device() != self.device or not shape or shape[-1] != cols \
                 or t.numel() != rows * cols:
             raise PtB200Error(f"{name}: needs {rows} rows of {cols} {dtype} on cuda:{self.device}, got "
                               f"{tuple(shape)} {t.dtype} on {t.device}")
+        if t.is_contiguous():
+            return t.data_ptr(), cols
         if len(shape) != 2:
             try:
                 t = t.view(rows, cols)
             except RuntimeError:
                 raise PtB200Error(f"{name}: its leading dimensions have no common row stride") from None
         ld, step = t.stride()
-        if step != 1 and cols > 1 and rows > 0:
+        if step != 1 and cols > 1:
             raise PtB200Error(f"{name}: its columns are not contiguous (stride {step})")
         if ld < cols:
             if rows > 1:
@@ -861,18 +864,13 @@ class Operators:
         return t.data_ptr(), ld
 
     def _vector(self, t, name: str, dtype, n: int) -> int:
-        """The address of a contiguous [n] tensor, 0 for None."""
+        """The address of a contiguous tensor of n elements, 0 for None."""
         if t is None:
             return 0
-        if t.dtype != dtype or t.get_device() != self.device or t.dim() != 1 or t.shape[0] != n \
-                or (n > 1 and t.stride(0) != 1):
+        if t.dtype != dtype or t.get_device() != self.device or t.numel() != n or not t.is_contiguous():
             raise PtB200Error(f"{name}: needs {n} contiguous {dtype} on cuda:{self.device}, got "
                               f"{tuple(t.shape)} {t.dtype} on {t.device}")
         return t.data_ptr()
-
-    def _flat(self, t, name: str, dtype, n: int) -> int:
-        """The address of a contiguous tensor of n elements, whatever its shape."""
-        return self._vector(t if t.dim() == 1 or not t.is_contiguous() else t.view(-1), name, dtype, n)
 
     def _act(self, act: str) -> int:
         code = self.ACTS.get(act)
@@ -880,14 +878,11 @@ class Operators:
             raise PtB200Error(f"act is one of {', '.join(self.ACTS)}, got {act!r}")
         return code
 
-    def _workspace(self, n: int):
-        return self._torch.empty(n, dtype=self._torch.uint8, device=self.device) if n else None
-
     def linear(self, x, w, bias=None, residual=None, act: str = "none", slope: float = 0.1,
                save_pre: bool = False):
         """act(x W^T + bias) + residual for x [..., in], w [out][in]; [..., out].  With save_pre
         also the value before the activation, as linear_backward wants it: (y, pre)."""
-        code, dt, empty = self._type(x, "x"), x.dtype, self._torch.empty
+        code, dt = self._type(x, "x"), x.dtype
         if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
             raise PtB200Error(f"linear: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit")
         n_out, n_in = w.shape
@@ -899,18 +894,19 @@ class Operators:
         bp = self._vector(bias, "bias", dt, n_out)
         rp, ldr = self._rows(residual, "residual", dt, rows, n_out) if residual is not None else (0, 0)
         shape = x.shape[:-1] + (n_out,)
-        y = empty(shape, dtype=dt, device=x.device)
-        pre = empty(shape, dtype=dt, device=x.device) if save_pre else None
+        y = x.new_empty(shape)
+        pre = self._torch.empty_like(y) if save_pre else None
+        a = self._act(act)
 
         def pack(work, nbytes):
-            return self._LINEAR.pack(code, self._act(act), rows, n_in, n_out, xp, wp, bp, rp,
+            return self._LINEAR.pack(code, a, rows, n_in, n_out, xp, wp, bp, rp,
                                      y.data_ptr(), pre.data_ptr() if save_pre else 0, ldx, ldw, ldr,
                                      n_out, n_out, work, nbytes, slope)
 
         args = pack(0, 0)
         need = self._lib.pt_b200_linear_work(self.h, args)
         if need:
-            work = self._workspace(need)
+            work = x.new_empty(need, dtype=self._torch.uint8)
             args = pack(work.data_ptr(), need)
         if self._lib.pt_b200_linear(self.h, self._stream(), args):
             _check(-1, "pt_b200_linear")
@@ -920,7 +916,7 @@ class Operators:
                         need_dx: bool = True, need_dw: bool = True, need_db: bool = True):
         """(dx, dw, db) of linear for dy [..., out]; None in the place of one not asked for.  pre is
         what linear(save_pre=True) kept, needed where there is an activation."""
-        code, dt, empty = self._type(dy, "dy"), dy.dtype, self._torch.empty
+        code, dt = self._type(dy, "dy"), dy.dtype
         if w.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != w.shape[0]:
             raise PtB200Error(f"linear_backward: dy {tuple(dy.shape)} and w {tuple(w.shape)} do not fit")
         n_out, n_in = w.shape
@@ -936,10 +932,9 @@ class Operators:
         xp, ldx = self._rows(x, "x", dt, rows, n_in)
         wp, ldw = self._rows(w, "w", dt, n_out, n_in)
         pp, ldp = self._rows(pre, "pre", dt, rows, n_out) if a else (0, 0)
-        dev = dy.device
-        dx = empty(dy.shape[:-1] + (n_in,), dtype=dt, device=dev) if need_dx else None
-        dw = empty((n_out, n_in), dtype=dt, device=dev) if need_dw else None
-        db = empty((n_out,), dtype=dt, device=dev) if need_db else None
+        dx = dy.new_empty(dy.shape[:-1] + (n_in,)) if need_dx else None
+        dw = dy.new_empty((n_out, n_in)) if need_dw else None
+        db = dy.new_empty((n_out,)) if need_db else None
 
         def pack(work, nbytes):
             return self._LINEAR_GRAD.pack(code, a, rows, n_in, n_out, gp, xp, wp, pp,
@@ -951,7 +946,7 @@ class Operators:
         args = pack(0, 0)
         need = self._lib.pt_b200_linear_backward_work(self.h, args)
         if need:
-            work = self._workspace(need)
+            work = dy.new_empty(need, dtype=self._torch.uint8)
             args = pack(work.data_ptr(), need)
         if self._lib.pt_b200_linear_backward(self.h, self._stream(), args):
             _check(-1, "pt_b200_linear_backward")
@@ -966,12 +961,11 @@ class Operators:
         rows = x.numel() // cols
         xp, ldx = self._rows(x, "x", dt, rows, cols)
         gp, bp = self._vector(gamma, "gamma", dt, cols), self._vector(beta, "beta", dt, cols)
-        y = torch.empty(x.shape, dtype=dt, device=x.device)
-        stat = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
-        mean, rstd = stat[0], stat[1]
-        sp = stat.data_ptr()
-        args = self._NORM.pack(code, eps, rows, cols, xp, gp, bp, y.data_ptr(), sp, sp + 4 * rows, ldx,
-                               cols)
+        y = torch.empty_like(x) if ldx == cols else x.new_empty(x.shape)
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
+        args = self._NORM.pack(code, eps, rows, cols, xp, gp, bp, y.data_ptr(), mean.data_ptr(),
+                               rstd.data_ptr(), ldx, cols)
         if self._lib.pt_b200_layer_norm(self.h, self._stream(), args):
             _check(-1, "pt_b200_layer_norm")
         return y, mean, rstd
@@ -979,25 +973,25 @@ class Operators:
     def layer_norm_backward(self, dy, x, gamma, mean, rstd, need_dx: bool = True,
                             need_dgamma: bool = True, need_dbeta: bool = True):
         """(dx, dgamma, dbeta) of layer_norm; None in the place of one not asked for."""
-        code, dt, empty = self._type(dy, "dy"), dy.dtype, self._torch.empty
+        code, dt = self._type(dy, "dy"), dy.dtype
         cols = dy.shape[-1] if dy.dim() else 0
         if cols == 0:
             raise PtB200Error(f"layer_norm_backward: dy {tuple(dy.shape)} has no columns")
         if not (need_dx or need_dgamma or need_dbeta):
             raise PtB200Error("layer_norm_backward: nothing to compute")
-        rows, dev = dy.numel() // cols, dy.device
+        rows = dy.numel() // cols
         yp, lddy = self._rows(dy, "dy", dt, rows, cols)
         xp, ldx = self._rows(x, "x", dt, rows, cols)
         gp = self._vector(gamma, "gamma", dt, cols)
         f32 = self._torch.float32
-        mp, rp = self._flat(mean, "mean", f32, rows), self._flat(rstd, "rstd", f32, rows)
-        dx = empty(dy.shape, dtype=dt, device=dev) if need_dx else None
-        dgamma = empty((cols,), dtype=dt, device=dev) if need_dgamma else None
-        dbeta = empty((cols,), dtype=dt, device=dev) if need_dbeta else None
+        mp, rp = self._vector(mean, "mean", f32, rows), self._vector(rstd, "rstd", f32, rows)
+        dx = (self._torch.empty_like(dy) if lddy == cols else dy.new_empty(dy.shape)) if need_dx else None
+        dgamma = dy.new_empty((cols,)) if need_dgamma else None
+        dbeta = dy.new_empty((cols,)) if need_dbeta else None
         need = 0
         if need_dgamma or need_dbeta:
             need = self._lib.pt_b200_layer_norm_backward_work(self.h, rows, cols)
-        work = self._workspace(need)
+        work = dy.new_empty(need, dtype=self._torch.uint8) if need else None
         args = self._NORM_GRAD.pack(code, 0, rows, cols, yp, xp, gp, mp, rp,
                                     dx.data_ptr() if need_dx else 0,
                                     dgamma.data_ptr() if need_dgamma else 0,
