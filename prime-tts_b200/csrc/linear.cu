@@ -221,7 +221,7 @@ extern "C" int pt_b200_linear(pt_b200_ops *h, void *stream, const pt_b200_linear
   q.k = p->in;
   q.e = epi;
   if (tc_prep(p->dtype, jobs, n, st)) return -1;
-  return tc_product(h, p->dtype, q, ColumnSums{}, n > 0, false, st);
+  return tc_products(h, p->dtype, &q, 1, ColumnSums{}, n > 0, st);
 }
 
 // The gradient's operand dpre is dy itself where nothing has to be computed or copied for it.
@@ -291,17 +291,11 @@ extern "C" int pt_b200_linear_backward(pt_b200_ops *h, void *stream, const pt_b2
     j.plane = g.plane;
     work += tc_plane_bytes(p->dtype, p->rows, p->out);
   }
-  TcProduct dx{}, dw{};
-  if (p->dx) dx.a = operand(h, p->dtype, p->w, p->out, p->in, p->ldw, &work, &jobs, &n);
-  if (p->dw) dw.a = operand(h, p->dtype, p->x, p->rows, p->in, p->ldx, &work, &jobs, &n);
-  ColumnSums sums{};
-  if (p->db) {
-    j.part = reinterpret_cast<float *>(work);
-    sums = ColumnSums{j.part, p->db, tc_row_blocks(h, p->rows, p->out), p->out};
-  }
-  if (j.dst || j.part) tc_add_job(h, p->dtype, &jobs, &n, j);
-  if (tc_prep(p->dtype, jobs, n, st)) return -1;
+  TcProduct products[2] = {};
+  int count = 0;
   if (p->dx) {
+    TcProduct &dx = products[count++];
+    dx.a = operand(h, p->dtype, p->w, p->out, p->in, p->ldw, &work, &jobs, &n);
     dx.b = g;
     dx.a_mn = true;
     dx.rows = p->rows;
@@ -309,10 +303,10 @@ extern "C" int pt_b200_linear_backward(pt_b200_ops *h, void *stream, const pt_b2
     dx.k = p->out;
     dx.e.y = p->dx;
     dx.e.ldy = p->lddx;
-    if (tc_product(h, p->dtype, dx, sums, n > 0, false, st)) return -1;
-    sums = ColumnSums{};
   }
   if (p->dw) {
+    TcProduct &dw = products[count++];
+    dw.a = operand(h, p->dtype, p->x, p->rows, p->in, p->ldx, &work, &jobs, &n);
     dw.b = g;
     dw.a_mn = dw.b_mn = true;
     dw.rows = p->out;
@@ -320,11 +314,15 @@ extern "C" int pt_b200_linear_backward(pt_b200_ops *h, void *stream, const pt_b2
     dw.k = p->rows;
     dw.e.y = p->dw;
     dw.e.ldy = p->lddw;
-    // dx and dW need the same passes and nothing of each other
-    if (tc_product(h, p->dtype, dw, sums, n > 0 || p->dx, p->dx != nullptr, st)) return -1;
-    sums = ColumnSums{};
   }
-  if (sums.parts == 0) return 0;
+  ColumnSums sums{};
+  if (p->db) {
+    j.part = reinterpret_cast<float *>(work);
+    sums = ColumnSums{j.part, p->db, tc_row_blocks(h, p->rows, p->out), p->out};
+  }
+  if (j.dst || j.part) tc_add_job(h, p->dtype, &jobs, &n, j);
+  if (tc_prep(p->dtype, jobs, n, st)) return -1;
+  if (count) return tc_products(h, p->dtype, products, count, sums, n > 0, st);
   return with_dtype(p->dtype, [&](auto *z) -> int {
     using T = std::remove_pointer_t<decltype(z)>;
     return reduce_columns<T>(sums.part, sums.parts, sums.n, static_cast<T *>(sums.out), st);

@@ -77,21 +77,33 @@ struct Divide {
 };
 constexpr int kBand = 16;
 
-struct TcArgs {
+// One product of a launch.
+struct TcOne {
   LinearEpi e;
   int64_t rows, chans;      // output rows (N side) and channels (M side)
   int kiters;               // k stages in all
-  int split;                // CTAs that share a tile's k range (the cluster)
-  int per;                  // k stages of one of them
+  int per;                  // k stages of one of the CTAs that share a tile's k range
   int bn;                   // rows per tile
-  int stages;
   int tiles_m, tiles_n;     // channel tiles, row tiles
   Divide by_band;           // by the tiles of a band
   Divide by_last;           // by the channel tiles of the last band, where it is not a whole one
   uint32_t idesc;
   bool a_mn, b_mn;
+};
+// One product, or two (the gradient's) whose tiles follow one another in the walk.
+constexpr int kMaxProducts = 2;
+struct TcArgs {
+  TcOne p[kMaxProducts];
+  int tiles0, tiles;        // the first product's, all of them
+  int split;                // CTAs that share a tile's k range (the cluster)
+  int stages;
+  uint32_t stage_bytes;
+  uint32_t acc_cols;        // TMEM columns from one accumulator to the next, a power of two
   bool beside;              // needs nothing of the kernel launched right before it
   ColumnSums sums;          // done beside the first tile, or parts = 0
+};
+struct TcMaps {
+  CUtensorMap a[kMaxProducts], b[kMaxProducts];
 };
 
 // ---- the same steps for one CTA (G = 1) and for a pair (G = 2, issued by its rank 0)
@@ -190,7 +202,7 @@ constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);   // atom, 
 
 // Tile t of the walk: channel tiles fastest inside bands of kBand, so that concurrent CTAs share
 // both operands through L2.
-__device__ __forceinline__ void tile_at(const TcArgs &g, int t, int *tm, int *tn) {
+__device__ __forceinline__ void tile_at(const TcOne &g, int t, int *tm, int *tn) {
   const int band = g.by_band.of(t);
   const int in = t - band * kBand * g.tiles_n;
   const bool last = (band + 1) * kBand > g.tiles_m;
@@ -240,16 +252,14 @@ __device__ __forceinline__ void emit16(const LinearEpi &e, float (&v)[16], int64
 // G CTAs to a tile, P planes per operand.
 template <class T, int G, int P>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                     const TcArgs g, uint32_t *gerr) {
+    linear_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs args, uint32_t *gerr) {
   namespace cg = cooperative_groups;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *gbase = smem_raw + (base - raw);
-  const int b_rows = g.bn / G;                     // rows of B in this CTA
-  const uint32_t a_plane = kM * KB * 2, b_plane = static_cast<uint32_t>(b_rows) * KB * 2;
-  const uint32_t stage_bytes = (P * (a_plane + b_plane) + 1023u) & ~1023u;
+  constexpr uint32_t a_plane = kM * KB * 2;
+  const uint32_t stage_bytes = args.stage_bytes, acc_cols = args.acc_cols;
   const uint32_t bar0 = base + kSmemBudget;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
@@ -260,13 +270,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  // accumulators are a power of two of columns apart, TMEM is allocated in powers of two from 32
-  uint32_t acc_cols = 16;
-  while (acc_cols < static_cast<uint32_t>(g.bn)) acc_cols *= 2;
   const uint32_t tmem_cols = 2 * acc_cols;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < g.stages; ++s) {
+    for (int s = 0; s < args.stages; ++s) {
       mbar_init(full(s), 2);
       mbar_init(empty(s), 1);
     }
@@ -279,8 +286,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
-    prefetch_tmap(&map_a);
-    prefetch_tmap(&map_b);
+    prefetch_tmap(&maps.a[0]);
+    prefetch_tmap(&maps.b[0]);
   }
   if (warp == 1) {
     alloc<G>(smem_u32(tmem_slot), tmem_cols);
@@ -292,7 +299,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t tmem = uniform(*tmem_slot);
 
   // What follows reads and writes global memory: after the kernels before this one.
-  if (!g.beside) wait_for_previous();
+  if (!args.beside) wait_for_previous();
   let_next_start();
 
   // The CTAs of a cluster work on a tile together: the pair, or those that share its k range.
@@ -300,12 +307,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   asm("mov.u32 %0, %%clusterid.x;" : "=r"(first));
   asm("mov.u32 %0, %%nclusterid.x;" : "=r"(step));
-  const int tiles = g.tiles_m * g.tiles_n;
   const int pair_rank = G == 2 ? rank : 0;
   const int k_rank = G == 2 ? 0 : rank;
-  const int k_lo = k_rank * g.per, k_hi = min(k_lo + g.per, g.kiters);
-  // stages per accumulator: all of them, or (three planes) one
-  const int chunk = P == 1 ? g.per : 1;
+  // tile t of the walk: its product, its place, and this CTA's stages of k
+  struct Tile {
+    const TcOne &g;
+    int tm, tn, k_lo, k_hi;
+  };
+  auto tile = [&](int t) -> Tile {
+    const int which = kMaxProducts > 1 && t >= args.tiles0;
+    const TcOne &g = args.p[which];
+    int tm, tn;
+    tile_at(g, t - (which ? args.tiles0 : 0), &tm, &tn);
+    const int k_lo = k_rank * g.per;
+    return Tile{g, tm, tn, k_lo, min(k_lo + g.per, g.kiters)};
+  };
 
   if (warp == 0 || warp == 2) {
     // ---------------- TMA producers: A in warp 0, B in warp 2 (a copy takes 80 to 120 clocks to issue)
@@ -313,16 +329,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const bool one = elect_one();
     int s = 0, issued = 0;
     uint32_t phase = 0, a0 = is_a ? base : base + P * a_plane;
-    const uint32_t plane = is_a ? a_plane : b_plane;
     // a pair's copies all count on rank 0's barrier, where the MMAs are issued
     const uint32_t bar0_of = G == 1 ? full(0) : in_rank0(full(0));
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step) {
-      int tm, tn;
-      tile_at(g, t, &tm, &tn);
-      const int chan0 = uniform((tm * G + pair_rank) * kM), row0 = uniform(tn * g.bn + pair_rank * b_rows);
-      for (int k = k_lo; k < k_hi; ++k) {
-        if (issued >= g.stages && !mbar_wait(empty(s), phase ^ 1u, abort_flag, gerr, ERR_WAIT_EMPTY)) {
+    for (int t = first; t < args.tiles && ok; t += step) {
+      const Tile at_tile = tile(t);
+      const TcOne &g = at_tile.g;
+      const CUtensorMap *map = t >= args.tiles0 ? (is_a ? &maps.a[1] : &maps.b[1]) : (is_a ? &maps.a[0] : &maps.b[0]);
+      const int b_rows = g.bn / G;                     // rows of B in this CTA
+      const uint32_t plane = is_a ? a_plane : static_cast<uint32_t>(b_rows) * KB * 2;
+      const int chan0 = uniform((at_tile.tm * G + pair_rank) * kM);
+      const int row0 = uniform(at_tile.tn * g.bn + pair_rank * b_rows);
+      for (int k = at_tile.k_lo; k < at_tile.k_hi; ++k) {
+        if (issued >= args.stages && !mbar_wait(empty(s), phase ^ 1u, abort_flag, gerr, ERR_WAIT_EMPTY)) {
           ok = false;
           break;
         }
@@ -336,31 +355,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int p = 0; p < P; ++p, at += a_plane) {
               if (g.a_mn) {
 #pragma unroll
-                for (int i = 0; i < kM / 64; ++i) load<G>(at + i * KB * 128, &map_a, bar, chan0 + i * 64, ku, p);
+                for (int i = 0; i < kM / 64; ++i) load<G>(at + i * KB * 128, map, bar, chan0 + i * 64, ku, p);
               } else {
-                load<G>(at, &map_a, bar, ku, chan0, p);
+                load<G>(at, map, bar, ku, chan0, p);
               }
             }
           } else {
 #pragma unroll
-            for (int p = 0; p < P; ++p, at += b_plane) {
+            for (int p = 0; p < P; ++p, at += plane) {
               if (g.b_mn) {
-                for (int i = 0; i < b_rows / 64; ++i) load<G>(at + i * KB * 128, &map_b, bar, row0 + i * 64, ku, p);
+                for (int i = 0; i < b_rows / 64; ++i) load<G>(at + i * KB * 128, map, bar, row0 + i * 64, ku, p);
               } else {
-                load<G>(at, &map_b, bar, ku, row0, p);
+                load<G>(at, map, bar, ku, row0, p);
               }
             }
           }
         }
         ++issued;
         a0 += stage_bytes;
-        if (++s == g.stages) s = 0, phase ^= 1u, a0 -= g.stages * stage_bytes;
+        if (++s == args.stages) s = 0, phase ^= 1u, a0 -= args.stages * stage_bytes;
       }
     }
     if (!ok && pair_rank == 0 && is_a) {   // copies in flight must land before shared memory is given up
-      const int flying = min(issued, g.stages);
+      const int flying = min(issued, args.stages);
       for (int i = 0; i < flying; ++i) {
-        if (s == 0) s = g.stages, phase ^= 1u;
+        if (s == 0) s = args.stages, phase ^= 1u;
         --s;
         uint32_t it = 0;
         while (!mbar_try_wait(full(s), phase) && ++it < kWaitLimit) {
@@ -372,15 +391,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     if (pair_rank == 0) {
       // ---------------- MMA issuer
       const bool one = elect_one();
-      const uint32_t a_adv = g.a_mn ? 2048u >> 4 : 32u >> 4;     // 16 elements of k further on
-      const uint32_t b_adv = g.b_mn ? 2048u >> 4 : 32u >> 4;
-      const uint32_t da0 = sdesc_lo(base, g.a_mn ? KB * 128 : 16);
-      const uint32_t db0 = sdesc_lo(base + P * a_plane, g.b_mn ? KB * 128 : 16);
       int s = 0, unit = 0;
       uint32_t phase = 0, at = 0;    // `at`: the stage's place, in the descriptors' 16 bytes
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        for (int k = k_lo; k < k_hi && ok; ++unit) {
+      for (int t = first; t < args.tiles && ok; t += step) {
+        const Tile at_tile = tile(t);
+        const TcOne &g = at_tile.g;
+        const uint32_t b_plane = static_cast<uint32_t>(g.bn / G) * KB * 2;
+        const uint32_t a_adv = g.a_mn ? 2048u >> 4 : 32u >> 4;     // 16 elements of k further on
+        const uint32_t b_adv = g.b_mn ? 2048u >> 4 : 32u >> 4;
+        const uint32_t da0 = sdesc_lo(base, g.a_mn ? KB * 128 : 16);
+        const uint32_t db0 = sdesc_lo(base + P * a_plane, g.b_mn ? KB * 128 : 16);
+        const int k_hi = at_tile.k_hi, chunk = P == 1 ? g.per : 1;   // stages per accumulator
+        for (int k = at_tile.k_lo; k < k_hi && ok; ++unit) {
           const int b = unit & 1;
           if (unit >= 2 && !mbar_wait(acc_empty(b), ((unit >> 1) & 1) ^ 1u, abort_flag, gerr, ERR_WAIT_ACC)) {
             ok = false;
@@ -415,7 +438,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             accumulate = 1;
             at += stage_bytes >> 4;
-            if (++s == g.stages) s = 0, phase ^= 1u, at = 0;
+            if (++s == args.stages) s = 0, phase ^= 1u, at = 0;
           }
           if (ok && one) commit<G>(acc_full(b));
         }
@@ -432,31 +455,31 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // ---------------- epilogue warps: lanes 32 (warp % 4) .. + 31, every fourth block of 16 columns
     const int quad = warp & 3, half = (warp - kFirstEpi) >> 2;
     const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    if (g.sums.parts > 0 && warp < kFirstEpi + kSumLanes) {   // column sums, 32 columns at a time, while the first tile's products run
+    if (args.sums.parts > 0 && warp < kFirstEpi + kSumLanes) {   // column sums, 32 columns at a time, while the first tile's products run
       float *red = reinterpret_cast<float *>(gbase + kSmemBudget + 512);
       const int row = warp - kFirstEpi;
-      for (int64_t c0 = blockIdx.x * 32; c0 < g.sums.n; c0 += gridDim.x * 32) {
+      for (int64_t c0 = blockIdx.x * 32; c0 < args.sums.n; c0 += gridDim.x * 32) {
         float v = 0.0f;
-        if (c0 + lane < g.sums.n)
+        if (c0 + lane < args.sums.n)
 #pragma unroll 4
-          for (int p = row; p < g.sums.parts; p += kSumLanes) v += g.sums.part[p * g.sums.n + c0 + lane];
+          for (int p = row; p < args.sums.parts; p += kSumLanes) v += args.sums.part[p * args.sums.n + c0 + lane];
         red[row * 33 + lane] = v;
         asm volatile("bar.sync 1, %0;" ::"n"(kSumLanes * 32) : "memory");
-        if (row == 0 && c0 + lane < g.sums.n) {
+        if (row == 0 && c0 + lane < args.sums.n) {
           v = 0.0f;
           for (int i = 0; i < kSumLanes; ++i) v += red[i * 33 + lane];
-          static_cast<T *>(g.sums.out)[c0 + lane] = from_f32<T>(v);
+          static_cast<T *>(args.sums.out)[c0 + lane] = from_f32<T>(v);
         }
         asm volatile("bar.sync 1, %0;" ::"n"(kSumLanes * 32) : "memory");
       }
     }
     int unit = 0;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step) {
-      int tm, tn;
-      tile_at(g, t, &tm, &tn);
-      const int64_t chan = static_cast<int64_t>(tm * G + pair_rank) * kM + quad * 32 + lane;
-      const int64_t row0 = static_cast<int64_t>(tn) * g.bn;
+    for (int t = first; t < args.tiles && ok; t += step) {
+      const Tile at_tile = tile(t);
+      const TcOne &g = at_tile.g;
+      const int64_t chan = static_cast<int64_t>(at_tile.tm * G + pair_rank) * kM + quad * 32 + lane;
+      const int64_t row0 = static_cast<int64_t>(at_tile.tn) * g.bn;
       const float bias = g.e.bias && chan < g.chans ? to_f32(static_cast<const T *>(g.e.bias)[chan]) : 0.0f;
       float *part = reinterpret_cast<float *>(gbase);   // split: [bn][128] of this CTA's part
       if constexpr (P == 1) {
@@ -466,7 +489,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int c = half * 16; c < g.bn; c += 64) {
           float v[16];
           tmem_ld16(tl + b * acc_cols + c, v);
-          if (g.split > 1) {
+          if (args.split > 1) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) part[(c + j) * kM + quad * 32 + lane] = v[j];
           } else {
@@ -484,7 +507,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < kMaxBn3 / 64; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-        for (int k = k_lo; k < k_hi && ok; k += chunk, ++unit) {
+        for (int k = at_tile.k_lo; k < at_tile.k_hi && ok; ++k, ++unit) {
           const int b = unit & 1;
           if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC)) {
             ok = false;
@@ -505,7 +528,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (lane == 0) arrive<G>(G == 1 ? acc_empty(b) : in_rank0(acc_empty(b)));
         }
         if (!ok) break;
-        if (g.split > 1) {
+        if (args.split > 1) {
           // the stages still hold operands of the last chunk until its MMAs are done, which the
           // last accumulator's arrival says
 #pragma unroll
@@ -528,26 +551,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   }
   __syncwarp();
-  if (G == 1 && g.split > 1) {
+  if (G == 1 && args.split > 1) {
     // ---------------- one tile per cluster: add the parts, a slice of the rows per CTA
     auto cluster = cg::this_cluster();
     cluster.sync();
     if (warp >= kFirstEpi && !*abort_flag) {
-      const int quad = warp & 3, half = (warp - kFirstEpi) >> 2;
-      int tm, tn;
-      tile_at(g, first, &tm, &tn);
-      const int64_t chan = static_cast<int64_t>(tm) * kM + quad * 32 + lane;
+      const int quad = warp & 3, half = (warp - kFirstEpi) >> 2, split = args.split;
+      const Tile at_tile = tile(first);
+      const TcOne &g = at_tile.g;
+      const int64_t chan = static_cast<int64_t>(at_tile.tm) * kM + quad * 32 + lane;
       float *part = reinterpret_cast<float *>(gbase);
-      const int width = g.bn / g.split;
+      const int width = g.bn / split;
       const float *from[kMaxSplit];
 #pragma unroll
       for (int r = 0; r < kMaxSplit; ++r)
-        from[r] = cluster.map_shared_rank(part, r < g.split ? r : 0) + quad * 32 + lane;
+        from[r] = cluster.map_shared_rank(part, r < split ? r : 0) + quad * 32 + lane;
       for (int c = rank * width + half; c < (rank + 1) * width; c += 4) {
-        const int64_t row = static_cast<int64_t>(tn) * g.bn + c;
+        const int64_t row = static_cast<int64_t>(at_tile.tn) * g.bn + c;
         float got[kMaxSplit], v = 0.0f;
 #pragma unroll
-        for (int r = 0; r < kMaxSplit; ++r) got[r] = r < g.split ? from[r][c * kM] : 0.0f;
+        for (int r = 0; r < kMaxSplit; ++r) got[r] = r < split ? from[r][c * kM] : 0.0f;
 #pragma unroll
         for (int r = 0; r < kMaxSplit; ++r) v += got[r];
         if (chan < g.chans && row < g.rows) linear_store<T>(g.e, row, chan, v);
@@ -563,7 +586,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     dealloc<G>(tmem, tmem_cols);
   }
   // a kernel that ran beside the one before it ends after it: the next may wait for this one alone
-  if (g.beside) wait_for_previous();
+  if (args.beside) wait_for_previous();
 }
 
 // ------------------------------------------------------------------------------ operand passes
@@ -706,6 +729,7 @@ int encode(CUtensorMap *m, const TcOperand &o, bool half, int planes, int box_in
 //   - a tile starts after 2800 and leaves after 300 + 15 bn, which the next tile hides;
 //   - parts of a split tile are exchanged in 3500 + 4 bn.
 // The clusters of a split must fit the GPU at once.
+inline int k_stages(int64_t k) { return static_cast<int>((k + KB - 1) / KB); }
 struct Shape {
   int group, bn, split;
 };
@@ -739,45 +763,52 @@ Shape pick_shape(const pt_b200_ops *h, int64_t rows, int64_t chans, int kiters, 
 }
 
 template <class T, int P>
-int launch(const pt_b200_ops *h, const TcProduct &p, const ColumnSums &sums, bool early, bool beside,
-           cudaStream_t st) {
-  TcArgs g{};
-  g.sums = sums;
-  g.beside = beside;
-  g.e = p.e;
-  g.rows = p.rows;
-  g.chans = p.chans;
-  g.a_mn = p.a_mn;
-  g.b_mn = p.b_mn;
-  g.kiters = static_cast<int>((p.k + KB - 1) / KB);
-  const Shape sh = pick_shape(h, p.rows, p.chans, g.kiters, P, p.b_mn);
-  const int G = sh.group;
-  g.bn = sh.bn;
-  g.split = sh.split;
-  g.per = (g.kiters + g.split - 1) / g.split;
-  const int stage = static_cast<int>(round_up(P * (kM + g.bn / G) * KB * 2, 1024));
-  g.stages = std::min(kMaxStages, kSmemBudget / stage);
-  g.tiles_m = static_cast<int>((p.chans + G * kM - 1) / (G * kM));
-  const int64_t tiles_n = (p.rows + g.bn - 1) / g.bn;
-  PTB_REQUIRE(tiles_n * g.tiles_m < (int64_t(1) << 29), "pt_b200: product of %lld x %lld is too large",
-              (long long)p.rows, (long long)p.chans);
-  g.tiles_n = static_cast<int>(tiles_n);
+int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes, int count, const ColumnSums &sums,
+           bool early, bool beside, cudaStream_t st) {
   constexpr bool kHalf = std::is_same_v<T, __half>;
-  const uint32_t fmt = kHalf ? 0u : 1u;
-  g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u) |
-            (static_cast<uint32_t>(g.bn >> 3) << 17) | (static_cast<uint32_t>(G * kM >> 4) << 24);
-  CUtensorMap ma, mb;
-  if (encode(&ma, p.a, kHalf, P, p.a_mn ? 64 : KB, p.a_mn ? KB : kM) ||
-      encode(&mb, p.b, kHalf, P, p.b_mn ? 64 : KB, p.b_mn ? KB : g.bn / G))
-    return -1;
+  const int G = shapes[0].group;
+  TcArgs a{};
+  TcMaps maps;
+  a.sums = sums;
+  a.beside = beside;
+  a.split = shapes[0].split;
+  a.acc_cols = 16;
+  for (int i = 0; i < count; ++i) {
+    const TcProduct &p = products[i];
+    TcOne &g = a.p[i];
+    g.e = p.e;
+    g.rows = p.rows;
+    g.chans = p.chans;
+    g.a_mn = p.a_mn;
+    g.b_mn = p.b_mn;
+    g.kiters = k_stages(p.k);
+    g.bn = shapes[i].bn;
+    g.per = (g.kiters + a.split - 1) / a.split;
+    g.tiles_m = static_cast<int>((p.chans + G * kM - 1) / (G * kM));
+    const int64_t tiles_n = (p.rows + g.bn - 1) / g.bn;
+    PTB_REQUIRE(tiles_n * g.tiles_m < (int64_t(1) << 29), "pt_b200: product of %lld x %lld is too large",
+                (long long)p.rows, (long long)p.chans);
+    g.tiles_n = static_cast<int>(tiles_n);
+    g.by_band = Divide(static_cast<uint32_t>(kBand * g.tiles_n));
+    g.by_last = Divide(g.tiles_m % kBand ? g.tiles_m % kBand : kBand);
+    const uint32_t fmt = kHalf ? 0u : 1u;
+    g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (p.a_mn ? 1u << 15 : 0u) | (p.b_mn ? 1u << 16 : 0u) |
+              (static_cast<uint32_t>(g.bn >> 3) << 17) | (static_cast<uint32_t>(G * kM >> 4) << 24);
+    if (encode(&maps.a[i], p.a, kHalf, P, p.a_mn ? 64 : KB, p.a_mn ? KB : kM) ||
+        encode(&maps.b[i], p.b, kHalf, P, p.b_mn ? 64 : KB, p.b_mn ? KB : g.bn / G))
+      return -1;
+    a.stage_bytes = std::max(a.stage_bytes, static_cast<uint32_t>(round_up(P * (kM + g.bn / G) * KB * 2, 1024)));
+    while (a.acc_cols < static_cast<uint32_t>(g.bn)) a.acc_cols *= 2;
+    if (i == 0) a.tiles0 = g.tiles_m * g.tiles_n;
+    a.tiles += g.tiles_m * g.tiles_n;
+  }
+  if (count == 1) maps.a[1] = maps.a[0], maps.b[1] = maps.b[0];
+  a.stages = std::min<int>(kMaxStages, kSmemBudget / a.stage_bytes);
   auto kernel = G == 1 ? linear_tc_kernel<T, 1, P> : linear_tc_kernel<T, 2, P>;
-  g.by_band = Divide(static_cast<uint32_t>(kBand * g.tiles_n));
-  g.by_last = Divide(g.tiles_m % kBand ? g.tiles_m % kBand : kBand);
-  const int64_t tiles = static_cast<int64_t>(g.tiles_m) * g.tiles_n;
-  const int group = G * g.split;
+  const int group = G * a.split;
+  const int at_once = group == 1 ? h->clusters[0] : group == 2 ? h->clusters[1] : a.tiles;
   cudaLaunchConfig_t cfg{};
-  const int64_t at_once = group == 1 ? h->clusters[0] : group == 2 ? h->clusters[1] : tiles;
-  cfg.gridDim = dim3(static_cast<unsigned>(group * std::min(tiles, at_once)));
+  cfg.gridDim = dim3(static_cast<unsigned>(group * (a.split > 1 ? a.tiles : std::min(a.tiles, at_once))));
   cfg.blockDim = dim3(kTcThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = st;
@@ -789,8 +820,25 @@ int launch(const pt_b200_ops *h, const TcProduct &p, const ColumnSums &sums, boo
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = early ? 2 : 1;
-  PTB_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, g, h->gerr));
+  PTB_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps, a, h->gerr));
   count_launch();
+  return 0;
+}
+
+template <class T, int P>
+int launch_products(const pt_b200_ops *h, const TcProduct *p, int count, ColumnSums sums, bool early,
+                    cudaStream_t st) {
+  Shape sh[kMaxProducts];
+  for (int i = 0; i < count; ++i) sh[i] = pick_shape(h, p[i].rows, p[i].chans, k_stages(p[i].k), P, p[i].b_mn);
+  // products of one kind of cluster share a launch (a split one only while its clusters all fit); the
+  // shape of each is its own, so that its sums are the same alone and in company
+  if (count == 2 && sh[0].group == sh[1].group && sh[0].split == 1 && sh[1].split == 1)
+    return launch<T, P>(h, p, sh, 2, sums, early, false, st);
+  for (int i = 0; i < count; ++i) {
+    // the second needs the same passes as the first, and nothing of it
+    if (launch<T, P>(h, p + i, sh + i, 1, sums, early || i, i > 0, st)) return -1;
+    sums = ColumnSums{};
+  }
   return 0;
 }
 
@@ -882,12 +930,12 @@ int tc_prep(int dtype, const PrepJobs &jobs, int n, cudaStream_t st) {
   });
 }
 
-int tc_product(const pt_b200_ops *h, int dtype, const TcProduct &p, const ColumnSums &sums, bool early, bool beside,
-               cudaStream_t st) {
+int tc_products(const pt_b200_ops *h, int dtype, const TcProduct *p, int count, const ColumnSums &sums, bool early,
+                cudaStream_t st) {
   switch (dtype) {
-    case PT_B200_F32: return launch<float, 3>(h, p, sums, early, beside, st);
-    case PT_B200_BF16: return launch<__nv_bfloat16, 1>(h, p, sums, early, beside, st);
-    default: return launch<__half, 1>(h, p, sums, early, beside, st);
+    case PT_B200_F32: return launch_products<float, 3>(h, p, count, sums, early, st);
+    case PT_B200_BF16: return launch_products<__nv_bfloat16, 1>(h, p, count, sums, early, st);
+    default: return launch_products<__half, 1>(h, p, count, sums, early, st);
   }
 }
 

@@ -67,10 +67,10 @@ TcOperand tc_planes(void *p, int64_t rows, int64_t cols);
 int tc_row_blocks(const pt_b200_ops *h, int64_t rows, int64_t cols);
 void tc_add_job(const pt_b200_ops *h, int dtype, PrepJobs *jobs, int *n, PrepJob job);
 int tc_prep(int dtype, const PrepJobs &jobs, int n, cudaStream_t st);
-// After a kernel of the same call that lets it start early, `early` hides the launch behind it;
-// `sums` is work that its epilogue warps do while the first tile's products run.  With `beside` the
-// product needs nothing of the kernel right before it, only of those before that one.
-int tc_product(const pt_b200_ops *h, int dtype, const TcProduct &p, const ColumnSums &sums, bool early, bool beside,
-               cudaStream_t st);
+// One product, or two that need nothing of each other.  After a kernel of the same call that lets
+// them start early, `early` hides the launch behind it; `sums` is work that epilogue warps do while
+// the first tile's products run.
+int tc_products(const pt_b200_ops *h, int dtype, const TcProduct *p, int count, const ColumnSums &sums, bool early,
+                cudaStream_t st);
 
 }  // namespace ptb

@@ -906,7 +906,7 @@ class Operators:
         args = pack(0, 0)
         need = self._lib.pt_b200_linear_work(self.h, args)
         if need:
-            work = x.new_empty(need, dtype=self._torch.uint8)
+            work = x.new_empty(-(-need // dt.itemsize))
             args = pack(work.data_ptr(), need)
         if self._lib.pt_b200_linear(self.h, self._stream(), args):
             _check(-1, "pt_b200_linear")
@@ -932,9 +932,15 @@ class Operators:
         xp, ldx = self._rows(x, "x", dt, rows, n_in)
         wp, ldw = self._rows(w, "w", dt, n_out, n_in)
         pp, ldp = self._rows(pre, "pre", dt, rows, n_out) if a else (0, 0)
-        dx = dy.new_empty(dy.shape[:-1] + (n_in,)) if need_dx else None
-        dw = dy.new_empty((n_out, n_in)) if need_dw else None
-        db = dy.new_empty((n_out,)) if need_db else None
+        new, like = dy.new_empty, self._torch.empty_like
+        # (empty_like is the cheaper call; a strided or reshaped tensor gets rows of its own)
+        dx = dw = db = None
+        if need_dx:
+            dx = like(x) if ldx == n_in and x.dim() == dy.dim() else new(dy.shape[:-1] + (n_in,))
+        if need_dw:
+            dw = like(w) if ldw == n_in else new((n_out, n_in))
+        if need_db:
+            db = new((n_out,))
 
         def pack(work, nbytes):
             return self._LINEAR_GRAD.pack(code, a, rows, n_in, n_out, gp, xp, wp, pp,
@@ -946,7 +952,7 @@ class Operators:
         args = pack(0, 0)
         need = self._lib.pt_b200_linear_backward_work(self.h, args)
         if need:
-            work = dy.new_empty(need, dtype=self._torch.uint8)
+            work = new(-(-need // dt.itemsize))
             args = pack(work.data_ptr(), need)
         if self._lib.pt_b200_linear_backward(self.h, self._stream(), args):
             _check(-1, "pt_b200_linear_backward")
@@ -991,7 +997,7 @@ class Operators:
         need = 0
         if need_dgamma or need_dbeta:
             need = self._lib.pt_b200_layer_norm_backward_work(self.h, rows, cols)
-        work = dy.new_empty(need, dtype=self._torch.uint8) if need else None
+        work = dy.new_empty(-(-need // dt.itemsize)) if need else None
         args = self._NORM_GRAD.pack(code, 0, rows, cols, yp, xp, gp, mp, rp,
                                     dx.data_ptr() if need_dx else 0,
                                     dgamma.data_ptr() if need_dgamma else 0,
