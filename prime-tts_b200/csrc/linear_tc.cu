@@ -51,7 +51,8 @@ constexpr int kEpiWarps = 16;   // four to a quarter of the lanes: two left an e
 constexpr int kFirstEpi = 3;
 constexpr int kTcThreads = (kFirstEpi + kEpiWarps) * 32;   // warps 0 and 2 copy A and B, warp 1 MMA, the rest epilogue
 constexpr int kM = 128;
-constexpr int kMaxBn1 = 256, kMaxBn3 = 192;   // rows per tile; three planes' sums are in registers
+constexpr uint32_t kTcWait = 1u << 21;   // tries of a wait inside a kernel that runs for milliseconds
+constexpr int kMaxBn1 = 256, kMaxBn3 = 128;   // rows per tile; three planes' sums are in registers
 constexpr int KB = 64;   // elements of k per stage: a 128-byte row
 constexpr int kMaxStages = 10;
 constexpr int kMaxSplit = 8;
@@ -229,15 +230,15 @@ __device__ __forceinline__ void emit16(const LinearEpi &e, float (&v)[16], int64
   if (e.residual) {
     const T *p = static_cast<const T *>(e.residual) + row0 * e.ldr + chan;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) r[j] = j < n ? to_f32(p[j * e.ldr]) : 0.0f;
+    for (int j = 0; j < 16; ++j, p += e.ldr) r[j] = j < n ? to_f32(*p) : 0.0f;
   }
 #pragma unroll
   for (int j = 0; j < 16; ++j) v[j] += bias;
   if (e.pre) {
     T *p = static_cast<T *>(e.pre) + row0 * e.ldp + chan;
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (j < n) p[j * e.ldp] = from_f32<T>(v[j]);
+    for (int j = 0; j < 16; ++j, p += e.ldp)
+      if (j < n) *p = from_f32<T>(v[j]);
   }
   with_act(e.act, ActOnAll{v, e.slope});
   if (e.residual) {
@@ -246,9 +247,10 @@ __device__ __forceinline__ void emit16(const LinearEpi &e, float (&v)[16], int64
   }
   T *p = static_cast<T *>(e.y) + row0 * e.ldy + chan;
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (j < n) p[j * e.ldy] = from_f32<T>(v[j]);
+  for (int j = 0; j < 16; ++j, p += e.ldy)
+    if (j < n) *p = from_f32<T>(v[j]);
 }
+
 // G CTAs to a tile, P planes per operand.
 template <class T, int G, int P>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -263,23 +265,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t bar0 = base + kSmemBudget;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+  // accumulators: two, or (three planes) two for each team of epilogue warps
+  constexpr int kBuffers = P == 1 ? 2 : 4;
   auto acc_full = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
-  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 2 + b); };   // rank 0's counts
-  const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 4);
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gbase + kSmemBudget + 8 * (2 * kMaxStages + 5));
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 4 + b); };   // rank 0's counts
+  const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 8);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gbase + kSmemBudget + 8 * (2 * kMaxStages + 9));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t tmem_cols = 2 * acc_cols;
+  const uint32_t tmem_cols = kBuffers * acc_cols;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < args.stages; ++s) {
       mbar_init(full(s), 2);
       mbar_init(empty(s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBuffers; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), G * kEpiWarps);
+      mbar_init(acc_empty(b), G * (P == 1 ? kEpiWarps : kEpiWarps / 2));
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int chan0 = uniform((at_tile.tm * G + pair_rank) * kM);
       const int row0 = uniform(at_tile.tn * g.bn + pair_rank * b_rows);
       for (int k = at_tile.k_lo; k < at_tile.k_hi; ++k) {
-        if (issued >= args.stages && !mbar_wait(empty(s), phase ^ 1u, abort_flag, gerr, ERR_WAIT_EMPTY)) {
+        if (issued >= args.stages && !mbar_wait(empty(s), phase ^ 1u, abort_flag, gerr, ERR_WAIT_EMPTY, kTcWait)) {
           ok = false;
           break;
         }
@@ -382,16 +386,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (s == 0) s = args.stages, phase ^= 1u;
         --s;
         uint32_t it = 0;
-        while (!mbar_try_wait(full(s), phase) && ++it < kWaitLimit) {
+        while (!mbar_try_wait(full(s), phase) && ++it < kTcWait) {
         }
-        if (it >= kWaitLimit && one) atomicOr(gerr, ERR_WAIT_DRAIN);
+        if (it >= kTcWait && one) atomicOr(gerr, ERR_WAIT_DRAIN);
       }
     }
   } else if (warp == 1) {
     if (pair_rank == 0) {
       // ---------------- MMA issuer
       const bool one = elect_one();
-      int s = 0, unit = 0;
+      int s = 0, turn = 0, units[2] = {0, 0};   // accumulators given to each team so far
       uint32_t phase = 0, at = 0;    // `at`: the stage's place, in the descriptors' 16 bytes
       bool ok = true;
       for (int t = first; t < args.tiles && ok; t += step) {
@@ -403,9 +407,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t da0 = sdesc_lo(base, g.a_mn ? KB * 128 : 16);
         const uint32_t db0 = sdesc_lo(base + P * a_plane, g.b_mn ? KB * 128 : 16);
         const int k_hi = at_tile.k_hi, chunk = P == 1 ? g.per : 1;   // stages per accumulator
+        const int team = P == 1 ? 0 : turn++ & 1;
+        int unit = team ? units[1] : units[0];
         for (int k = at_tile.k_lo; k < k_hi && ok; ++unit) {
-          const int b = unit & 1;
-          if (unit >= 2 && !mbar_wait(acc_empty(b), ((unit >> 1) & 1) ^ 1u, abort_flag, gerr, ERR_WAIT_ACC)) {
+          const int b = 2 * team + (unit & 1);
+          if (unit >= 2 && !mbar_wait(acc_empty(b), ((unit >> 1) & 1) ^ 1u, abort_flag, gerr, ERR_WAIT_ACC, kTcWait)) {
             ok = false;
             break;
           }
@@ -414,7 +420,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int k_end = min(k + chunk, k_hi);
           uint32_t accumulate = 0;
           for (; k < k_end; ++k) {
-            if (!mbar_wait(full(s), phase, abort_flag, gerr, ERR_WAIT_FULL)) {
+            if (!mbar_wait(full(s), phase, abort_flag, gerr, ERR_WAIT_FULL, kTcWait)) {
               ok = false;
               break;
             }
@@ -442,18 +448,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           if (ok && one) commit<G>(acc_full(b));
         }
+        (team ? units[1] : units[0]) = unit;
       }
       if (!ok) {   // MMAs already issued must finish before TMEM is released
         if (one) commit<G>(drain);
         uint32_t it = 0;
-        while (!mbar_try_wait(drain, 0) && ++it < kWaitLimit) {
+        while (!mbar_try_wait(drain, 0) && ++it < kTcWait) {
         }
-        if (it >= kWaitLimit && one) atomicOr(gerr, ERR_WAIT_DRAIN);
+        if (it >= kTcWait && one) atomicOr(gerr, ERR_WAIT_DRAIN);
       }
     }
   } else {
     // ---------------- epilogue warps: lanes 32 (warp % 4) .. + 31, every fourth block of 16 columns
-    const int quad = warp & 3, half = (warp - kFirstEpi) >> 2;
+    const int part_of = warp - kFirstEpi, quad = warp & 3, team = part_of >> 3;
     const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     if (args.sums.parts > 0 && warp < kFirstEpi + kSumLanes) {   // column sums, 32 columns at a time, while the first tile's products run
       float *red = reinterpret_cast<float *>(gbase + kSmemBudget + 512);
@@ -473,7 +480,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         asm volatile("bar.sync 1, %0;" ::"n"(kSumLanes * 32) : "memory");
       }
     }
-    int unit = 0;
+    int unit = 0, turn = 0;
     bool ok = true;
     for (int t = first; t < args.tiles && ok; t += step) {
       const Tile at_tile = tile(t);
@@ -484,9 +491,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       float *part = reinterpret_cast<float *>(gbase);   // split: [bn][128] of this CTA's part
       if constexpr (P == 1) {
         const int b = unit & 1;
-        if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC)) break;
+        if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC, kTcWait)) break;
         tc_fence_after();
-        for (int c = half * 16; c < g.bn; c += 64) {
+        for (int c = (part_of >> 2) * 16; c < g.bn; c += 64) {
           float v[16];
           tmem_ld16(tl + b * acc_cols + c, v);
           if (args.split > 1) {
@@ -502,23 +509,28 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) arrive<G>(G == 1 ? acc_empty(b) : in_rank0(acc_empty(b)));
         ++unit;
       } else {
-        float acc[kMaxBn3 / 64][16];
+        // Two teams of eight warps take turns at the tiles: one adds up the chunks of a tile while the
+        // other still stores the one before (19434 x 192 x 768 spent 4700 of a tile's 7900 clocks on
+        // its stores with one team).
+        if (turn++ % 2 != team) continue;
+        const int half = (part_of & 7) >> 2;
+        float acc[kMaxBn3 / 32][16];
 #pragma unroll
-        for (int i = 0; i < kMaxBn3 / 64; ++i)
+        for (int i = 0; i < kMaxBn3 / 32; ++i)
 #pragma unroll
           for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
         for (int k = at_tile.k_lo; k < at_tile.k_hi && ok; ++k, ++unit) {
-          const int b = unit & 1;
-          if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC)) {
+          const int b = 2 * team + (unit & 1);
+          if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC, kTcWait)) {
             ok = false;
             break;
           }
           tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < kMaxBn3 / 64; ++i) {
-            if (half * 16 + i * 64 < g.bn) {
+          for (int i = 0; i < kMaxBn3 / 32; ++i) {
+            if (half * 16 + i * 32 < g.bn) {
               float v[16];
-              tmem_ld16(tl + b * acc_cols + half * 16 + i * 64, v);
+              tmem_ld16(tl + b * acc_cols + half * 16 + i * 32, v);
 #pragma unroll
               for (int j = 0; j < 16; ++j) acc[i][j] += v[j];
             }
@@ -532,15 +544,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // the stages still hold operands of the last chunk until its MMAs are done, which the
           // last accumulator's arrival says
 #pragma unroll
-          for (int i = 0; i < kMaxBn3 / 64; ++i)
-            if (half * 16 + i * 64 < g.bn)
+          for (int i = 0; i < kMaxBn3 / 32; ++i)
+            if (half * 16 + i * 32 < g.bn)
 #pragma unroll
               for (int j = 0; j < 16; ++j)
-                part[(half * 16 + i * 64 + j) * kM + quad * 32 + lane] = acc[i][j];
+                part[(half * 16 + i * 32 + j) * kM + quad * 32 + lane] = acc[i][j];
         } else {
 #pragma unroll
-          for (int i = 0; i < kMaxBn3 / 64; ++i) {
-            const int c = half * 16 + i * 64;
+          for (int i = 0; i < kMaxBn3 / 32; ++i) {
+            const int c = half * 16 + i * 32;
             const int n = static_cast<int>(min(static_cast<int64_t>(16), g.rows - row0 - c));
             if (c < g.bn && chan < g.chans && n > 0) {
               emit16<T>(g.e, acc[i], chan, row0 + c, n, bias);

@@ -58,8 +58,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 // Bounded wait.  Returns false when the limit ran out or another role already aborted; the
 // first to give up raises the CTA abort flag and ORs `err` into the global error word.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag,
-                                          uint32_t *gerr, uint32_t err) {
-  for (uint32_t it = 0; it < kWaitLimit; ++it) {
+                                          uint32_t *gerr, uint32_t err, uint32_t limit = kWaitLimit) {
+  for (uint32_t it = 0; it < limit; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort_flag) return false;
   }
