@@ -784,6 +784,28 @@ class Decoder:
 
 
 # --------------------------------------------------------------------------------------------
+TORCH_MODULE_PATH = os.path.join(HERE, "_pt_b200_torch.so")
+_torch_mod = None
+
+
+def _torch_module():
+    """The operators' entry points on torch tensors (csrc/torch_ops.cpp; raises if not built)."""
+    global _torch_mod
+    if _torch_mod is None:
+        if not os.path.exists(TORCH_MODULE_PATH):
+            raise FileNotFoundError(f"{TORCH_MODULE_PATH} is missing: run `make -C {HERE}`")
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries first)
+        lib()
+        spec = importlib.util.spec_from_file_location("_pt_b200_torch", TORCH_MODULE_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.set_error_class(PtB200Error)
+        _torch_mod = mod
+    return _torch_mod
+
+
 class Operators:
     """The transformer-layer operators on torch CUDA tensors (pt_b200_ops_*): the linear layer with
     its fused epilogue and the layer norm, forward and backward.
@@ -795,27 +817,20 @@ class Operators:
     raises PtB200Error before anything is launched; sync() waits and reports device errors."""
 
     ACTS = {"none": 0, "leaky": 1, "relu": 2, "gelu": 5, "silu": 6}
-    # the argument structs of include/pt_b200.h, packed field by field
+    # the argument structs of include/pt_b200.h, packed field by field, for calls of the C entries
     _LINEAR = struct.Struct("=2i3q4Q2Q5qQqf4x")
     _LINEAR_GRAD = struct.Struct("=2i3q4Q3Q6qQqf4x")
     _NORM = struct.Struct("=if2q3QQ2Q2q")
     _NORM_GRAD = struct.Struct("=2i2q3Q2Q3Q3qQq")
 
     def __init__(self, device: int = 0):
-        import torch
-        self._torch = torch
-        self._lib = lib()
         self.h = None
+        self._lib, self._call = lib(), _torch_module()
         h = self._lib.pt_b200_ops_create(device)
         if not h:
             _check(-1, "pt_b200_ops_create")
         self.h = h
         self.device = device
-        self._types = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-        # torch's current stream as a handle; its Stream object costs a microsecond to make
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        self._stream = (lambda: raw(device)) if raw else (
-            lambda: torch.cuda.current_stream(device).cuda_stream)
 
     def close(self) -> None:
         if self.h:
@@ -832,45 +847,9 @@ class Operators:
         """Wait for torch's current stream and report device errors."""
         _check(self._lib.pt_b200_ops_sync(self.h, self._stream()), "pt_b200_ops_sync")
 
-    def _type(self, t, what: str) -> int:
-        """The element type of a call's first tensor."""
-        code = self._types.get(t.dtype)
-        if code is None or t.get_device() != self.device:
-            raise PtB200Error(f"{what}: needs a float32, bfloat16 or float16 tensor on cuda:"
-                              f"{self.device}, got {t.dtype} on {t.device}")
-        return code
-
-    def _rows(self, t, name: str, dtype, rows: int, cols: int):
-        """(address, row stride) of a [..., cols] tensor seen as [rows][cols]."""
-        shape = t.shape
-        if t.dtype != dtype or t.get_device() != self.device or not shape or shape[-1] != cols \
-                or t.numel() != rows * cols:
-            raise PtB200Error(f"{name}: needs {rows} rows of {cols} {dtype} on cuda:{self.device}, got "
-                              f"{tuple(shape)} {t.dtype} on {t.device}")
-        if t.is_contiguous():
-            return t.data_ptr(), cols
-        if len(shape) != 2:
-            try:
-                t = t.view(rows, cols)
-            except RuntimeError:
-                raise PtB200Error(f"{name}: its leading dimensions have no common row stride") from None
-        ld, step = t.stride()
-        if step != 1 and cols > 1:
-            raise PtB200Error(f"{name}: its columns are not contiguous (stride {step})")
-        if ld < cols:
-            if rows > 1:
-                raise PtB200Error(f"{name}: its rows overlap (stride {ld} for {cols} columns)")
-            ld = cols
-        return t.data_ptr(), ld
-
-    def _vector(self, t, name: str, dtype, n: int) -> int:
-        """The address of a contiguous tensor of n elements, 0 for None."""
-        if t is None:
-            return 0
-        if t.dtype != dtype or t.get_device() != self.device or t.numel() != n or not t.is_contiguous():
-            raise PtB200Error(f"{name}: needs {n} contiguous {dtype} on cuda:{self.device}, got "
-                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
-        return t.data_ptr()
+    def _stream(self) -> int:
+        import torch
+        return torch.cuda.current_stream(self.device).cuda_stream
 
     def _act(self, act: str) -> int:
         code = self.ACTS.get(act)
@@ -882,127 +861,22 @@ class Operators:
                save_pre: bool = False):
         """act(x W^T + bias) + residual for x [..., in], w [out][in]; [..., out].  With save_pre
         also the value before the activation, as linear_backward wants it: (y, pre)."""
-        code, dt = self._type(x, "x"), x.dtype
-        if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[1]:
-            raise PtB200Error(f"linear: x {tuple(x.shape)} and w {tuple(w.shape)} do not fit")
-        n_out, n_in = w.shape
-        if n_in == 0 or n_out == 0:
-            raise PtB200Error(f"linear: w {tuple(w.shape)} is empty")
-        rows = x.numel() // n_in
-        xp, ldx = self._rows(x, "x", dt, rows, n_in)
-        wp, ldw = self._rows(w, "w", dt, n_out, n_in)
-        bp = self._vector(bias, "bias", dt, n_out)
-        rp, ldr = self._rows(residual, "residual", dt, rows, n_out) if residual is not None else (0, 0)
-        shape = x.shape[:-1] + (n_out,)
-        y = x.new_empty(shape)
-        pre = self._torch.empty_like(y) if save_pre else None
-        a = self._act(act)
-
-        def pack(work, nbytes):
-            return self._LINEAR.pack(code, a, rows, n_in, n_out, xp, wp, bp, rp,
-                                     y.data_ptr(), pre.data_ptr() if save_pre else 0, ldx, ldw, ldr,
-                                     n_out, n_out, work, nbytes, slope)
-
-        args = pack(0, 0)
-        need = self._lib.pt_b200_linear_work(self.h, args)
-        if need:
-            work = x.new_empty(-(-need // dt.itemsize))
-            args = pack(work.data_ptr(), need)
-        if self._lib.pt_b200_linear(self.h, self._stream(), args):
-            _check(-1, "pt_b200_linear")
-        return (y, pre) if save_pre else y
+        return self._call.linear(self.h or 0, self.device, x, w, bias, residual, self._act(act), slope,
+                                 save_pre)
 
     def linear_backward(self, dy, x, w, pre=None, act: str = "none", slope: float = 0.1,
                         need_dx: bool = True, need_dw: bool = True, need_db: bool = True):
         """(dx, dw, db) of linear for dy [..., out]; None in the place of one not asked for.  pre is
         what linear(save_pre=True) kept, needed where there is an activation."""
-        code, dt = self._type(dy, "dy"), dy.dtype
-        if w.dim() != 2 or dy.dim() < 1 or dy.shape[-1] != w.shape[0]:
-            raise PtB200Error(f"linear_backward: dy {tuple(dy.shape)} and w {tuple(w.shape)} do not fit")
-        n_out, n_in = w.shape
-        if n_in == 0 or n_out == 0:
-            raise PtB200Error(f"linear_backward: w {tuple(w.shape)} is empty")
-        if not (need_dx or need_dw or need_db):
-            raise PtB200Error("linear_backward: nothing to compute")
-        rows = dy.numel() // n_out
-        a = self._act(act)
-        if a and pre is None:
-            raise PtB200Error(f"linear_backward: act {act!r} needs pre")
-        gp, lddy = self._rows(dy, "dy", dt, rows, n_out)
-        xp, ldx = self._rows(x, "x", dt, rows, n_in)
-        wp, ldw = self._rows(w, "w", dt, n_out, n_in)
-        pp, ldp = self._rows(pre, "pre", dt, rows, n_out) if a else (0, 0)
-        new, like = dy.new_empty, self._torch.empty_like
-        # (empty_like is the cheaper call; a strided or reshaped tensor gets rows of its own)
-        dx = dw = db = None
-        if need_dx:
-            dx = like(x) if ldx == n_in and x.dim() == dy.dim() else new(dy.shape[:-1] + (n_in,))
-        if need_dw:
-            dw = like(w) if ldw == n_in else new((n_out, n_in))
-        if need_db:
-            db = new((n_out,))
-
-        def pack(work, nbytes):
-            return self._LINEAR_GRAD.pack(code, a, rows, n_in, n_out, gp, xp, wp, pp,
-                                          dx.data_ptr() if need_dx else 0,
-                                          dw.data_ptr() if need_dw else 0,
-                                          db.data_ptr() if need_db else 0, lddy, ldx, ldw, ldp,
-                                          n_in, n_in, work, nbytes, slope)
-
-        args = pack(0, 0)
-        need = self._lib.pt_b200_linear_backward_work(self.h, args)
-        if need:
-            work = new(-(-need // dt.itemsize))
-            args = pack(work.data_ptr(), need)
-        if self._lib.pt_b200_linear_backward(self.h, self._stream(), args):
-            _check(-1, "pt_b200_linear_backward")
-        return dx, dw, db
+        return self._call.linear_backward(self.h or 0, self.device, dy, x, w, pre, self._act(act), slope,
+                                          need_dx, need_dw, need_db)
 
     def layer_norm(self, x, gamma=None, beta=None, eps: float = 1e-5):
         """Layer norm over the last dimension: (y, mean, rstd), the statistics in float32."""
-        code, dt, torch = self._type(x, "x"), x.dtype, self._torch
-        cols = x.shape[-1] if x.dim() else 0
-        if cols == 0:
-            raise PtB200Error(f"layer_norm: x {tuple(x.shape)} has no columns")
-        rows = x.numel() // cols
-        xp, ldx = self._rows(x, "x", dt, rows, cols)
-        gp, bp = self._vector(gamma, "gamma", dt, cols), self._vector(beta, "beta", dt, cols)
-        y = torch.empty_like(x) if ldx == cols else x.new_empty(x.shape)
-        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
-        rstd = torch.empty_like(mean)
-        args = self._NORM.pack(code, eps, rows, cols, xp, gp, bp, y.data_ptr(), mean.data_ptr(),
-                               rstd.data_ptr(), ldx, cols)
-        if self._lib.pt_b200_layer_norm(self.h, self._stream(), args):
-            _check(-1, "pt_b200_layer_norm")
-        return y, mean, rstd
+        return self._call.layer_norm(self.h or 0, self.device, x, gamma, beta, eps)
 
     def layer_norm_backward(self, dy, x, gamma, mean, rstd, need_dx: bool = True,
                             need_dgamma: bool = True, need_dbeta: bool = True):
         """(dx, dgamma, dbeta) of layer_norm; None in the place of one not asked for."""
-        code, dt = self._type(dy, "dy"), dy.dtype
-        cols = dy.shape[-1] if dy.dim() else 0
-        if cols == 0:
-            raise PtB200Error(f"layer_norm_backward: dy {tuple(dy.shape)} has no columns")
-        if not (need_dx or need_dgamma or need_dbeta):
-            raise PtB200Error("layer_norm_backward: nothing to compute")
-        rows = dy.numel() // cols
-        yp, lddy = self._rows(dy, "dy", dt, rows, cols)
-        xp, ldx = self._rows(x, "x", dt, rows, cols)
-        gp = self._vector(gamma, "gamma", dt, cols)
-        f32 = self._torch.float32
-        mp, rp = self._vector(mean, "mean", f32, rows), self._vector(rstd, "rstd", f32, rows)
-        dx = (self._torch.empty_like(dy) if lddy == cols else dy.new_empty(dy.shape)) if need_dx else None
-        dgamma = dy.new_empty((cols,)) if need_dgamma else None
-        dbeta = dy.new_empty((cols,)) if need_dbeta else None
-        need = 0
-        if need_dgamma or need_dbeta:
-            need = self._lib.pt_b200_layer_norm_backward_work(self.h, rows, cols)
-        work = dy.new_empty(-(-need // dt.itemsize)) if need else None
-        args = self._NORM_GRAD.pack(code, 0, rows, cols, yp, xp, gp, mp, rp,
-                                    dx.data_ptr() if need_dx else 0,
-                                    dgamma.data_ptr() if need_dgamma else 0,
-                                    dbeta.data_ptr() if need_dbeta else 0, lddy, ldx, cols,
-                                    work.data_ptr() if need else 0, need)
-        if self._lib.pt_b200_layer_norm_backward(self.h, self._stream(), args):
-            _check(-1, "pt_b200_layer_norm_backward")
-        return dx, dgamma, dbeta
+        return self._call.layer_norm_backward(self.h or 0, self.device, dy, x, gamma, mean, rstd, need_dx,
+                                              need_dgamma, need_dbeta)

@@ -58,3 +58,22 @@ def test_null_handles_are_refused():
 def test_no_such_device():
     with pytest.raises(pt_b200.PtB200Error, match="out of range"):
         pt_b200.Operators(device=63)
+
+
+def test_cpu_tensors_are_refused():
+    """The torch entry points turn a tensor elsewhere down before the handle is used; there is no CPU
+    path."""
+    torch = pytest.importorskip("torch")
+    call, t = pt_b200._torch_module(), torch.zeros(2, 4)
+    for fn, args in (("linear", (t, t, None, None, 0, 0.1, False)),
+                     ("linear_backward", (t, t, t, None, 0, 0.1, True, True, True)),
+                     ("layer_norm", (t, None, None, 1e-5)),
+                     ("layer_norm_backward", (t, t, None, t, t, True, True, True))):
+        with pytest.raises(pt_b200.PtB200Error, match="on cuda:0, got torch.float32 on cpu"):
+            getattr(call, fn)(1, 0, *args)
+        with pytest.raises(pt_b200.PtB200Error, match="have been closed"):
+            getattr(call, fn)(0, 0, *args)
+        with pytest.raises(pt_b200.PtB200Error, match="needs a tensor"):
+            getattr(call, fn)(1, 0, None, *args[1:])
+        with pytest.raises(TypeError, match="arguments are needed"):
+            getattr(call, fn)(1, 0)
