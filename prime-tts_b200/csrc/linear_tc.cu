@@ -91,11 +91,14 @@ struct TcOne {
   uint32_t idesc;
   bool a_mn, b_mn;
 };
-// One product, or two (the gradient's) whose tiles follow one another in the walk.
+// One product, or two (the gradient's).  Worker w of W (a CTA, a pair, a cluster) takes tiles w, w + W,
+// ... of the first product, whose tiles are the longer ones; then all workers take the second's in
+// turns, but after `both` turns only those that had one tile less of the first, from `late` on.
 constexpr int kMaxProducts = 2;
 struct TcArgs {
   TcOne p[kMaxProducts];
-  int tiles0, tiles;        // the first product's, all of them
+  int tiles[kMaxProducts];
+  int both, late;
   int split;                // CTAs that share a tile's k range (the cluster)
   int stages;
   uint32_t stage_bytes;
@@ -313,18 +316,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   asm("mov.u32 %0, %%nclusterid.x;" : "=r"(step));
   const int pair_rank = G == 2 ? rank : 0;
   const int k_rank = G == 2 ? 0 : rank;
-  // tile t of the walk: its product, its place, and this CTA's stages of k
+  // the n-th tile of this worker: its product, its place, and this CTA's stages of k
   struct Tile {
     const TcOne &g;
-    int tm, tn, k_lo, k_hi;
+    int which, tm, tn, k_lo, k_hi;
   };
-  auto tile = [&](int t) -> Tile {
-    const int which = kMaxProducts > 1 && t >= args.tiles0;
+  const int longs = first < args.tiles[0] ? (args.tiles[0] - first - 1) / step + 1 : 0;
+  auto place = [&](int n, int *which) -> int {   // -1: no more
+    *which = n >= longs;
+    if (!*which) return first + n * step;
+    const int turn = n - longs;
+    if (turn >= args.both && first < args.late) return -1;
+    const int t = turn < args.both ? turn * step + first
+                                   : args.both * step + (turn - args.both) * (step - args.late) + first - args.late;
+    return t < args.tiles[1] ? t : -1;
+  };
+  auto tile = [&](int t, int which) -> Tile {
     const TcOne &g = args.p[which];
     int tm, tn;
-    tile_at(g, t - (which ? args.tiles0 : 0), &tm, &tn);
+    tile_at(g, t, &tm, &tn);
     const int k_lo = k_rank * g.per;
-    return Tile{g, tm, tn, k_lo, min(k_lo + g.per, g.kiters)};
+    return Tile{g, which, tm, tn, k_lo, min(k_lo + g.per, g.kiters)};
   };
 
   if (warp == 0 || warp == 2) {
@@ -336,10 +348,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // a pair's copies all count on rank 0's barrier, where the MMAs are issued
     const uint32_t bar0_of = G == 1 ? full(0) : in_rank0(full(0));
     bool ok = true;
-    for (int t = first; t < args.tiles && ok; t += step) {
-      const Tile at_tile = tile(t);
+    for (int n = 0, t, which; ok && (t = place(n, &which)) >= 0; ++n) {
+      const Tile at_tile = tile(t, which);
       const TcOne &g = at_tile.g;
-      const CUtensorMap *map = t >= args.tiles0 ? (is_a ? &maps.a[1] : &maps.b[1]) : (is_a ? &maps.a[0] : &maps.b[0]);
+      const CUtensorMap *map = is_a ? &maps.a[which] : &maps.b[which];
       const int b_rows = g.bn / G;                     // rows of B in this CTA
       const uint32_t plane = is_a ? a_plane : static_cast<uint32_t>(b_rows) * KB * 2;
       const int chan0 = uniform((at_tile.tm * G + pair_rank) * kM);
@@ -398,8 +410,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int s = 0, turn = 0, units[2] = {0, 0};   // accumulators given to each team so far
       uint32_t phase = 0, at = 0;    // `at`: the stage's place, in the descriptors' 16 bytes
       bool ok = true;
-      for (int t = first; t < args.tiles && ok; t += step) {
-        const Tile at_tile = tile(t);
+      for (int n = 0, t, which; ok && (t = place(n, &which)) >= 0; ++n) {
+        const Tile at_tile = tile(t, which);
         const TcOne &g = at_tile.g;
         const uint32_t b_plane = static_cast<uint32_t>(g.bn / G) * KB * 2;
         const uint32_t a_adv = g.a_mn ? 2048u >> 4 : 32u >> 4;     // 16 elements of k further on
@@ -482,8 +494,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     int unit = 0, turn = 0;
     bool ok = true;
-    for (int t = first; t < args.tiles && ok; t += step) {
-      const Tile at_tile = tile(t);
+    for (int n = 0, t, which; ok && (t = place(n, &which)) >= 0; ++n) {
+      const Tile at_tile = tile(t, which);
       const TcOne &g = at_tile.g;
       const int64_t chan = static_cast<int64_t>(at_tile.tm * G + pair_rank) * kM + quad * 32 + lane;
       const int64_t row0 = static_cast<int64_t>(at_tile.tn) * g.bn;
@@ -569,7 +581,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     cluster.sync();
     if (warp >= kFirstEpi && !*abort_flag) {
       const int quad = warp & 3, half = (warp - kFirstEpi) >> 2, split = args.split;
-      const Tile at_tile = tile(first);
+      const Tile at_tile = tile(first, 0);
       const TcOne &g = at_tile.g;
       const int64_t chan = static_cast<int64_t>(at_tile.tm) * kM + quad * 32 + lane;
       float *part = reinterpret_cast<float *>(gbase);
@@ -811,16 +823,30 @@ int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes,
       return -1;
     a.stage_bytes = std::max(a.stage_bytes, static_cast<uint32_t>(round_up(P * (kM + g.bn / G) * KB * 2, 1024)));
     while (a.acc_cols < static_cast<uint32_t>(g.bn)) a.acc_cols *= 2;
-    if (i == 0) a.tiles0 = g.tiles_m * g.tiles_n;
-    a.tiles += g.tiles_m * g.tiles_n;
+    a.tiles[i] = g.tiles_m * g.tiles_n;
   }
   if (count == 1) maps.a[1] = maps.a[0], maps.b[1] = maps.b[0];
   a.stages = std::min<int>(kMaxStages, kSmemBudget / a.stage_bytes);
   auto kernel = G == 1 ? linear_tc_kernel<T, 1, P> : linear_tc_kernel<T, 2, P>;
   const int group = G * a.split;
-  const int at_once = group == 1 ? h->clusters[0] : group == 2 ? h->clusters[1] : a.tiles;
+  const int all = a.tiles[0] + a.tiles[1];
+  const int workers = a.split > 1 ? all : std::min(all, group == 1 ? h->clusters[0] : h->clusters[1]);
+  // the turns that all workers take part in: those that end the call soonest
+  const int busy = a.tiles[0] % workers;   // workers with one long tile more
+  a.both = a.tiles[1];
+  if (count == 2 && busy) {
+    const double c0 = a.p[0].kiters * static_cast<double>(a.p[0].bn), c1 = a.p[1].kiters * static_cast<double>(a.p[1].bn);
+    double best = 0;
+    for (int both = 0; both <= (a.tiles[1] + workers - 1) / workers; ++both) {
+      const int left = std::max(0, a.tiles[1] - both * workers);
+      const int more = (left + workers - busy - 1) / (workers - busy);
+      const double end = std::max(c0 + both * c1, (both + more) * c1);
+      if (both == 0 || end < best) best = end, a.both = both;
+    }
+    a.late = busy;
+  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(group * (a.split > 1 ? a.tiles : std::min(a.tiles, at_once))));
+  cfg.gridDim = dim3(static_cast<unsigned>(group * workers));
   cfg.blockDim = dim3(kTcThreads);
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = st;
@@ -844,8 +870,12 @@ int launch_products(const pt_b200_ops *h, const TcProduct *p, int count, ColumnS
   for (int i = 0; i < count; ++i) sh[i] = pick_shape(h, p[i].rows, p[i].chans, k_stages(p[i].k), P, p[i].b_mn);
   // products of one kind of cluster share a launch (a split one only while its clusters all fit); the
   // shape of each is its own, so that its sums are the same alone and in company
-  if (count == 2 && sh[0].group == sh[1].group && sh[0].split == 1 && sh[1].split == 1)
-    return launch<T, P>(h, p, sh, 2, sums, early, false, st);
+  if (count == 2 && sh[0].group == sh[1].group && sh[0].split == 1 && sh[1].split == 1) {
+    const bool swap = k_stages(p[1].k) * static_cast<double>(sh[1].bn) > k_stages(p[0].k) * static_cast<double>(sh[0].bn);
+    const TcProduct two[2] = {p[swap], p[!swap]};   // longer tiles first
+    const Shape shapes[2] = {sh[swap], sh[!swap]};
+    return launch<T, P>(h, two, shapes, 2, sums, early, false, st);
+  }
   for (int i = 0; i < count; ++i) {
     // the second needs the same passes as the first, and nothing of it
     if (launch<T, P>(h, p + i, sh + i, 1, sums, early || i, i > 0, st)) return -1;
