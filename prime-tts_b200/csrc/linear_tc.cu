@@ -615,8 +615,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 // ------------------------------------------------------------------------------ operand passes
 constexpr int kPrepBlock = 256;
-constexpr int kPrepRows = 2;   // rows a thread has in flight
-constexpr int kPrepPerSm = 3;  // blocks of a pass that run on one SM at once, and that it is cut into
+constexpr int kPrepRows = 1;   // rows a thread has in flight: 2 and 4 cost blocks of an SM and were 8 to 40% slower
+constexpr int kPrepPerSm = 4;  // blocks of a pass that run on one SM at once, and that it is cut into
 
 template <class T>
 struct Eight {
