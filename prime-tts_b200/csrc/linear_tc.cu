@@ -35,6 +35,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "linear_tc.cuh"
 #include "ptx.cuh"
@@ -756,10 +757,11 @@ int encode(CUtensorMap *m, const TcOperand &o, bool half, int planes, int box_in
 inline int k_stages(int64_t k) { return static_cast<int>((k + KB - 1) / KB); }
 struct Shape {
   int group, bn, split;
+  double clocks;   // of the call, and of one tile in a walk
+  double tile;
 };
 Shape pick_shape(const pt_b200_ops *h, int64_t rows, int64_t chans, int kiters, int planes, bool b_mn) {
-  Shape best{0, 0, 1};
-  double best_cost = 0;
+  Shape best{0, 0, 1, 0, 0};
   const int products = planes == 1 ? 1 : 6;
   for (int group : {1, 2}) {
     const int64_t tm = (chans + group * kM - 1) / (group * kM);
@@ -779,7 +781,7 @@ Shape pick_shape(const pt_b200_ops *h, int64_t rows, int64_t chans, int kiters, 
         const int64_t at_once = group == 2 ? h->clusters[1] : h->clusters[log];
         const int64_t waves = (tiles + at_once - 1) / at_once;
         const double cost = 2800 + waves * std::max(per * stage, leave) + leave + (split > 1 ? 3500 + 4.0 * bn : 0);
-        if (!best.bn || cost < best_cost) best = Shape{group, bn, split}, best_cost = cost;
+        if (!best.bn || cost < best.clocks) best = Shape{group, bn, split, cost, std::max(per * stage, leave)};
       }
     }
   }
@@ -788,7 +790,7 @@ Shape pick_shape(const pt_b200_ops *h, int64_t rows, int64_t chans, int kiters, 
 
 template <class T, int P>
 int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes, int count, const ColumnSums &sums,
-           bool early, bool beside, cudaStream_t st) {
+           bool early, bool beside, int most, cudaStream_t st) {
   constexpr bool kHalf = std::is_same_v<T, __half>;
   const int G = shapes[0].group;
   TcArgs a{};
@@ -830,7 +832,7 @@ int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes,
   auto kernel = G == 1 ? linear_tc_kernel<T, 1, P> : linear_tc_kernel<T, 2, P>;
   const int group = G * a.split;
   const int all = a.tiles[0] + a.tiles[1];
-  const int workers = a.split > 1 ? all : std::min(all, group == 1 ? h->clusters[0] : h->clusters[1]);
+  const int workers = a.split > 1 ? all : std::min({all, most, group == 1 ? h->clusters[0] : h->clusters[1]});
   // the turns that all workers take part in: those that end the call soonest
   const int busy = a.tiles[0] % workers;   // workers with one long tile more
   a.both = a.tiles[1];
@@ -874,11 +876,24 @@ int launch_products(const pt_b200_ops *h, const TcProduct *p, int count, ColumnS
     const bool swap = k_stages(p[1].k) * static_cast<double>(sh[1].bn) > k_stages(p[0].k) * static_cast<double>(sh[0].bn);
     const TcProduct two[2] = {p[swap], p[!swap]};   // longer tiles first
     const Shape shapes[2] = {sh[swap], sh[!swap]};
-    return launch<T, P>(h, two, shapes, 2, sums, early, false, st);
+    return launch<T, P>(h, two, shapes, 2, sums, early, false, INT_MAX, st);
   }
+  // Otherwise one after the other, which start together where there is room: the second needs the same
+  // passes as the first and nothing of it.  A split product leaves SMs free, so it goes first, and the
+  // other keeps to those SMs if it is done there in the meantime.
+  const bool swap = count == 2 && sh[1].split > sh[0].split;
   for (int i = 0; i < count; ++i) {
-    // the second needs the same passes as the first, and nothing of it
-    if (launch<T, P>(h, p + i, sh + i, 1, sums, early || i, i > 0, st)) return -1;
+    const int at = swap ? 1 - i : i;
+    int most = INT_MAX;
+    if (i == 1 && sh[1 - at].split > 1 && sh[at].split == 1) {
+      const TcProduct &q = p[1 - at], &mine = p[at];
+      const int64_t busy = (q.chans + kM - 1) / kM * ((q.rows + sh[1 - at].bn - 1) / sh[1 - at].bn) * sh[1 - at].split;
+      const int64_t room = (h->sms - busy) / sh[at].group;
+      const int64_t tiles = (mine.chans + sh[at].group * kM - 1) / (sh[at].group * kM) *
+                            ((mine.rows + sh[at].bn - 1) / sh[at].bn);
+      if (room > 0 && (tiles + room - 1) / room * sh[at].tile < sh[1 - at].clocks) most = static_cast<int>(room);
+    }
+    if (launch<T, P>(h, p + at, sh + at, 1, sums, early || i, i > 0, most, st)) return -1;
     sums = ColumnSums{};
   }
   return 0;
