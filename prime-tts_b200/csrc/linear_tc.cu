@@ -620,7 +620,7 @@ constexpr int kPrepRows = 1;   // rows a thread has in flight: 2 and 4 cost bloc
 constexpr int kPrepPerSm = 4;  // blocks of a pass that run on one SM at once, and that it is cut into
 
 template <class T>
-struct Eight {
+struct alignas(16) Eight {
   T v[8];
 };
 template <class T>
@@ -629,7 +629,7 @@ __device__ __forceinline__ void load8(const T *p, int n, bool vec, Eight<T> *o) 
     constexpr int V = 16 / sizeof(T);
 #pragma unroll
     for (int i = 0; i < 8 / V; ++i)
-      *reinterpret_cast<Pack<T, V> *>(o->v + i * V) = *reinterpret_cast<const Pack<T, V> *>(p + i * V);
+      *reinterpret_cast<uint4 *>(o->v + i * V) = __ldcs(reinterpret_cast<const uint4 *>(p + i * V));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o->v[i] = i < n ? p[i] : from_f32<T>(0.0f);
@@ -812,7 +812,8 @@ int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes,
     g.per = (g.kiters + a.split - 1) / a.split;
     g.tiles_m = static_cast<int>((p.chans + G * kM - 1) / (G * kM));
     const int64_t tiles_n = (p.rows + g.bn - 1) / g.bn;
-    PTB_REQUIRE(tiles_n * g.tiles_m < (int64_t(1) << 29), "pt_b200: product of %lld x %lld is too large",
+    PTB_REQUIRE(tiles_n * g.tiles_m < (int64_t(1) << 29) && tiles_n < (int64_t(1) << 26),
+                "pt_b200: product of %lld x %lld is too large",
                 (long long)p.rows, (long long)p.chans);
     g.tiles_n = static_cast<int>(tiles_n);
     g.by_band = Divide(static_cast<uint32_t>(kBand * g.tiles_n));
