@@ -20,7 +20,7 @@ struct ActOnOne {
   float &v;
   float slope;
   template <int ACT>
-  __device__ __forceinline__ void operator()() const { v = act_value<ACT>(v, slope); }
+  __device__ __forceinline__ void operator()() const { v = act_value<ACT>(both(v), slope).x; }
 };
 template <class T>
 __device__ __forceinline__ void linear_store(const LinearEpi &e, int64_t m, int64_t n, float v) {

@@ -224,7 +224,10 @@ struct ActOnAll {
   __device__ __forceinline__ void operator()() const {
     if constexpr (ACT != PT_B200_ACT_NONE)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = act_value<ACT>(v[j], slope);
+      for (int j = 0; j < 16; j += 2) {
+        const float2 o = act_value<ACT>(make_float2(v[j], v[j + 1]), slope);
+        v[j] = o.x, v[j + 1] = o.y;
+      }
   }
 };
 template <class T>
@@ -642,7 +645,7 @@ struct PrepRows {
   const PrepJob &a;
   int64_t c, r0, step;
   int n;
-  float (&sum)[8];
+  float2 (&sum)[4];
   template <int ACT>
   __device__ __forceinline__ void operator()() const {
     for (int64_t r1 = r0; r1 < a.rows; r1 += kPrepRows * step) {
@@ -662,12 +665,12 @@ struct PrepRows {
         if (r >= a.rows) break;
         float d[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          d[i] = to_f32(s[u].v[i]);
-          // (explicit operations: a sum must not depend on what else is made of d)
+        for (int i = 0; i < 8; i += 2) {
+          float2 t = make_float2(to_f32(s[u].v[i]), to_f32(s[u].v[i + 1]));
           if constexpr (ACT != PT_B200_ACT_NONE)
-            d[i] = __fmul_rn(d[i], act_grad<ACT>(to_f32(p[u].v[i]), a.slope));
-          sum[i] = __fadd_rn(sum[i], d[i]);
+            t = mul2(t, act_grad<ACT>(make_float2(to_f32(p[u].v[i]), to_f32(p[u].v[i + 1])), a.slope));
+          sum[i / 2] = add2(sum[i / 2], t);
+          d[i] = t.x, d[i + 1] = t.y;
         }
         if (!a.dst) continue;
         if constexpr (sizeof(T) == 4) {
@@ -700,7 +703,7 @@ struct PrepRows {
 // where rows are aligned.
 template <class T>
 __global__ void __launch_bounds__(kPrepBlock, kPrepPerSm) prep_kernel(const __grid_constant__ PrepJobs jobs) {
-  __shared__ float red[kPrepBlock * 8];
+  __shared__ __align__(8) float red[kPrepBlock * 8];
   let_next_start();
   int job = 0, block = blockIdx.x;
 #pragma unroll
@@ -711,7 +714,7 @@ __global__ void __launch_bounds__(kPrepBlock, kPrepPerSm) prep_kernel(const __gr
   const int cb = block % a.col_blocks, rb = block / a.col_blocks;
   const int64_t c = (static_cast<int64_t>(cb) * a.lanes + tx) * 8;
   const int n = static_cast<int>(min(static_cast<int64_t>(8), a.cols - c));
-  float sum[8] = {};
+  float2 sum[4] = {};
   if (n > 0)
     with_act(a.act, PrepRows<T>{a, c, static_cast<int64_t>(rb) * height + ty,
                                 static_cast<int64_t>(a.row_blocks) * height, n, sum});
@@ -719,7 +722,7 @@ __global__ void __launch_bounds__(kPrepBlock, kPrepPerSm) prep_kernel(const __gr
   // the block's row lanes, added in order
   const int width = a.lanes * 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) red[ty * width + tx * 8 + i] = sum[i];
+  for (int i = 0; i < 4; ++i) *reinterpret_cast<float2 *>(red + ty * width + tx * 8 + 2 * i) = sum[i];
   __syncthreads();
   for (int i = threadIdx.x; i < width; i += kPrepBlock) {
     const int64_t col = static_cast<int64_t>(cb) * width + i;

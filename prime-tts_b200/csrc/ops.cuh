@@ -67,6 +67,33 @@ int with_dtype(int dtype, F &&fn) {
 }
 inline int dtype_bytes(int dtype) { return dtype == PT_B200_F32 ? 4 : 2; }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // ---- activations.  A NaN passes through each of them; the slope of relu and leaky at 0 is that
 // of the side the comparison puts it on (relu 0, leaky 1).
 //
@@ -90,45 +117,55 @@ __device__ __forceinline__ float rcp_fast(float x) {
 }
 constexpr float kLog2E = 1.4426950408889634f;
 
-__device__ __forceinline__ void normal_cdf(float p, float *cdf, float *gauss) {
-  const float e = exp2_fast(p * p * (-0.5f * kLog2E));
-  const float t = rcp_fast(fmaf(0.3275911f * kSqrtHalf, fabsf(p), 1.0f));
-  float q = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);   // (half the polynomial)
-  q = fmaf(q, t, 0.5f * 1.421413741f);
-  q = fmaf(q, t, 0.5f * -0.284496736f);
-  q = fmaf(q, t, 0.5f * 0.254829592f);
-  const float h = q * t * e;
-  *cdf = p < 0.0f ? h : 1.0f - h;
+__device__ __forceinline__ void normal_cdf(float2 p, float2 *cdf, float2 *gauss) {
+  const float2 a = mul2(mul2(p, p), both(-0.5f * kLog2E));
+  const float2 e = make_float2(exp2_fast(a.x), exp2_fast(a.y));
+  const float2 d = fma2(both(0.3275911f * kSqrtHalf), make_float2(fabsf(p.x), fabsf(p.y)), both(1.0f));
+  const float2 t = make_float2(rcp_fast(d.x), rcp_fast(d.y));
+  float2 q = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));   // (half the polynomial)
+  q = fma2(q, t, both(0.5f * 1.421413741f));
+  q = fma2(q, t, both(0.5f * -0.284496736f));
+  q = fma2(q, t, both(0.5f * 0.254829592f));
+  // 1/2 - h(|p|) / 2 takes the sign of p: cdf - 1/2
+  const float2 c = fma2(mul2(q, t), make_float2(-e.x, -e.y), both(0.5f));
+  *cdf = add2(make_float2(copysignf(c.x, p.x), copysignf(c.y, p.y)), both(0.5f));
   *gauss = e;
 }
 
+// Value and slope of two arguments at once.
 template <int ACT>
-__device__ __forceinline__ float act_value(float p, float slope) {
-  if constexpr (ACT == PT_B200_ACT_LEAKY) return p < 0.0f ? slope * p : p;
-  if constexpr (ACT == PT_B200_ACT_RELU) return p < 0.0f ? 0.0f : p;
+__device__ __forceinline__ float2 act_value(float2 p, float slope) {
+  if constexpr (ACT == PT_B200_ACT_LEAKY)
+    return make_float2(p.x < 0.0f ? slope * p.x : p.x, p.y < 0.0f ? slope * p.y : p.y);
+  if constexpr (ACT == PT_B200_ACT_RELU) return make_float2(p.x < 0.0f ? 0.0f : p.x, p.y < 0.0f ? 0.0f : p.y);
   if constexpr (ACT == PT_B200_ACT_GELU) {
-    float cdf, gauss;
+    float2 cdf, gauss;
     normal_cdf(p, &cdf, &gauss);
-    return p * cdf;
+    return mul2(p, cdf);
   }
-  if constexpr (ACT == PT_B200_ACT_SILU) return p * rcp_fast(1.0f + exp2_fast(p * -kLog2E));
+  if constexpr (ACT == PT_B200_ACT_SILU) {
+    const float2 a = mul2(p, both(-kLog2E));
+    return mul2(p, make_float2(rcp_fast(1.0f + exp2_fast(a.x)), rcp_fast(1.0f + exp2_fast(a.y))));
+  }
   return p;
 }
 
 template <int ACT>
-__device__ __forceinline__ float act_grad(float p, float slope) {
-  if constexpr (ACT == PT_B200_ACT_LEAKY) return p < 0.0f ? slope : 1.0f;
-  if constexpr (ACT == PT_B200_ACT_RELU) return p <= 0.0f ? 0.0f : 1.0f;
+__device__ __forceinline__ float2 act_grad(float2 p, float slope) {
+  if constexpr (ACT == PT_B200_ACT_LEAKY) return make_float2(p.x < 0.0f ? slope : 1.0f, p.y < 0.0f ? slope : 1.0f);
+  if constexpr (ACT == PT_B200_ACT_RELU) return make_float2(p.x <= 0.0f ? 0.0f : 1.0f, p.y <= 0.0f ? 0.0f : 1.0f);
   if constexpr (ACT == PT_B200_ACT_GELU) {
-    float cdf, gauss;
+    float2 cdf, gauss;
     normal_cdf(p, &cdf, &gauss);
-    return fmaf(p * kInvSqrt2Pi, gauss, cdf);
+    return fma2(mul2(p, both(kInvSqrt2Pi)), gauss, cdf);
   }
   if constexpr (ACT == PT_B200_ACT_SILU) {
-    const float s = rcp_fast(1.0f + exp2_fast(p * -kLog2E));
-    return s * (1.0f + p * (1.0f - s));
+    const float2 a = mul2(p, both(-kLog2E));
+    const float2 s = make_float2(rcp_fast(1.0f + exp2_fast(a.x)), rcp_fast(1.0f + exp2_fast(a.y)));
+    // s (1 + p (1 - s))
+    return fma2(mul2(s, p), add2(both(1.0f), make_float2(-s.x, -s.y)), s);
   }
-  return 1.0f;
+  return both(1.0f);
 }
 
 // fn.template operator()<ACT>() for the activation's code: the choice is made once, outside loops.
