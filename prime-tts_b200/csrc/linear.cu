@@ -23,11 +23,10 @@ struct FewArgs {
 // bound by the weights' bytes, and by its latency where they are few.  A warp takes two channels and a
 // share of k: it reads 16 bytes of each weight row and of each row of x (which stays in L1) per lane
 // and step, kAhead steps in flight with no branch between the loads, and adds up in fp32 FMAs.
-// Lanes, then the warps that share a channel's k, add up in a fixed order.  Measured against the
-// tensor cores (tc): bf16, 4096 to 1024, 4 rows 5.6 us (tc 6.8), 8 rows 7.5 (6.8); 4096 to 4096, 2
-// rows 8.0 (8.7), 4 rows 11.1 (8.7); fp32, which the tensor cores need in planes first, 4096 to 4096,
-// 8 rows 17.4 (48).
-constexpr int kFewGroup = 8, kFewWarps = 8, kFewChans = 2, kFewFill = 16;
+// Lanes, then the warps that share a channel's k, add up in a fixed order.  More rows than eight are
+// groups of eight, which read the weights again from L2.  1 x 4096 x 4096 bf16 5.8 us (5.8 TB/s), 8 x
+// 4096 x 4096 fp32 15.6 us; with twice as many warps, in two waves, 6.9 and 22.9.
+constexpr int kFewGroup = 8, kFewWarps = 8, kFewChans = 2, kFewFill = 8;
 
 // Sums of v[0 .. N) over the warp, by halves: N / 2 + N / 4 + ... exchanges, not 5 N.  Lane l holds
 // the sum of value (l / (32 / N)).
@@ -48,7 +47,7 @@ __device__ __forceinline__ float warp_sums(float (&v)[N], int lane) {
 }
 
 template <class T, int R, bool VEC>
-__global__ void __launch_bounds__(kFewWarps * 32) linear_few_kernel(const FewArgs a) {
+__global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const FewArgs a) {
   constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1, kAhead = VEC ? (R <= 2 ? 4 : R == 4 ? 2 : 1) : 4;
   constexpr int kSums = kFewChans * R;
   using P = Pack<T, V>;
@@ -117,13 +116,14 @@ int launch_few(const pt_b200_ops *h, const FewArgs &args, cudaStream_t st) {
   // share a channel's k among warps until there are kFewFill on every SM, or a share is a single step
   const int64_t teams = (a.out + kFewChans - 1) / kFewChans;
   a.shares = 1;
-  while (a.shares < kFewWarps && teams * a.shares < kFewFill * h->sms && a.in > a.shares * 32 * V) a.shares *= 2;
+  const int64_t groups = (a.rows + kFewGroup - 1) / kFewGroup;
+  while (a.shares < kFewWarps && teams * groups * a.shares < kFewFill * h->sms && a.in > a.shares * 32 * V) a.shares *= 2;
   const int64_t per_block = kFewWarps / a.shares;
   const unsigned blocks = static_cast<unsigned>((teams + per_block - 1) / per_block);
   auto *kernel = a.rows == 1 ? linear_few_kernel<T, 1, VEC>
                  : a.rows == 2 ? linear_few_kernel<T, 2, VEC>
                  : a.rows <= 4 ? linear_few_kernel<T, 4, VEC> : linear_few_kernel<T, 8, VEC>;
-  kernel<<<dim3(blocks, (a.rows + kFewGroup - 1) / kFewGroup), kFewWarps * 32, 0, st>>>(a);
+  kernel<<<dim3(blocks, static_cast<unsigned>(groups)), kFewWarps * 32, 0, st>>>(a);
   PTB_CUDA(cudaGetLastError());
   count_launch();
   return 0;
@@ -156,13 +156,23 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
          n_out < (int64_t(1) << 30);
 }
 
-// Whether a call takes the few-rows kernel: while its FMAs cost less than what the tensor cores need
-// beside their products (a start, and planes where the operands cannot be read where they lie).
+// Whether a call takes the few-rows kernel: by the microseconds that both would take, linear in the
+// weights w = in x out and in the FMAs rows x w (fits to measurements, the tensor cores' in brackets;
+// rows x in x out):
+//   bf16  4 x 4096 x 1024 4.5 (6.8), 8 x 1024 x 1024 3.9 (5.9), 8 x 4096 x 1024 7.0 (7.1), 2 x 4096 x
+//         4096 7.4 (8.8), 4 x 4096 x 4096 10.5 (8.8), 16 x 1024 x 1024 5.0 (6.0), 64 x 192 x 768 5.7 (4.9)
+//   not aligned, so that the tensor cores need copies: 4 x 4001 x 4001 16.3 (21), 8 x 4001 x 4001 25.6 (21),
+//         64 x 193 x 515 4.5 (6.2), 32 x 1001 x 1001 9.6 (8.3)
+//   fp32, which the tensor cores need in planes: 8 x 1024 x 1024 3.7 (9.7), 8 x 4096 x 4096 15.6 (48),
+//         16 x 192 x 768 3.2 (8.7), 64 x 1024 x 1024 10.6 (11.4)
+constexpr int kFewRows = 64;
 bool few_rows(const pt_b200_linear_args *p) {
-  if (p->dtype == PT_B200_F32) return p->rows <= 2 * kFewGroup;
-  const bool direct = tc_direct(p->dtype, p->x, p->rows, p->ldx) && tc_direct(p->dtype, p->w, p->out, p->ldw);
-  if (!direct) return p->rows <= kFewGroup / 2 || (p->rows <= kFewGroup && p->in * p->out <= (1 << 22));
-  return p->rows <= 2 || (p->rows <= 4 && p->in * p->out <= (1 << 22));
+  if (p->rows > kFewRows) return false;
+  const double w = static_cast<double>(p->in) * static_cast<double>(p->out) * 1e-6, fma = w * p->rows;
+  if (p->dtype == PT_B200_F32) return 2.4 + fma / 10 < 8.5 + 2.4 * w;
+  if (tc_direct(p->dtype, p->x, p->rows, p->ldx) && tc_direct(p->dtype, p->w, p->out, p->ldw))
+    return 2.4 + fma / 6 < 5.7 + 0.18 * w;
+  return 2.4 + fma / 4.5 < 8 + 0.8 * w;
 }
 
 }  // namespace
