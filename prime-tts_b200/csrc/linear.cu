@@ -156,23 +156,27 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
          n_out < (int64_t(1) << 30);
 }
 
-// Whether a call takes the few-rows kernel: by the microseconds that both would take, linear in the
-// weights w = in x out and in the FMAs rows x w (fits to measurements, the tensor cores' in brackets;
-// rows x in x out):
-//   bf16  4 x 4096 x 1024 4.5 (6.8), 8 x 1024 x 1024 3.9 (5.9), 8 x 4096 x 1024 7.0 (7.1), 2 x 4096 x
-//         4096 7.4 (8.8), 4 x 4096 x 4096 10.5 (8.8), 16 x 1024 x 1024 5.0 (6.0), 64 x 192 x 768 5.7 (4.9)
-//   not aligned, so that the tensor cores need copies: 4 x 4001 x 4001 16.3 (21), 8 x 4001 x 4001 25.6 (21),
-//         64 x 193 x 515 4.5 (6.2), 32 x 1001 x 1001 9.6 (8.3)
-//   fp32, which the tensor cores need in planes: 8 x 1024 x 1024 3.7 (9.7), 8 x 4096 x 4096 15.6 (48),
-//         16 x 192 x 768 3.2 (8.7), 64 x 1024 x 1024 10.6 (11.4)
-constexpr int kFewRows = 64;
+// Whether a call takes the few-rows kernel: by the microseconds that both would take.  Its own follow
+// from its warps' tasks (two channels x eight rows), each a start and k; the tensor cores' from a start,
+// the weights and the first stages of k.  Fits to measurements (the tensor cores' in brackets, rows x
+// in x out):
+//   bf16  4 x 4096 x 1024 4.5 (6.8), 8 x 1024 x 1024 3.9 (5.9), 2 x 4096 x 4096 7.4 (8.8), 4 x 4096 x
+//         4096 10.5 (8.8), 64 x 192 x 768 5.7 (4.9), 1000 x 64 x 64 6.2 (4.5)
+//   not aligned, so that the tensor cores need copies: 128 x 101 x 201 4.4 (5.9), 500 x 101 x 201 10.1
+//         (5.9), 4 x 4001 x 4001 16.3 (21), 8 x 4001 x 4001 25.6 (21)
+//   fp32, which the tensor cores need in planes: 8 x 4096 x 4096 15.6 (48), 16 x 192 x 768 3.2 (8.7),
+//         128 x 768 x 192 5.3 (9.9), 2000 x 192 x 16 3.3 (9.4), 1000 x 192 x 192 14.1 (9.4)
+constexpr int kFewRows = 4096;
 bool few_rows(const pt_b200_linear_args *p) {
   if (p->rows > kFewRows) return false;
-  const double w = static_cast<double>(p->in) * static_cast<double>(p->out) * 1e-6, fma = w * p->rows;
-  if (p->dtype == PT_B200_F32) return 2.4 + fma / 10 < 8.5 + 2.4 * w;
-  if (tc_direct(p->dtype, p->x, p->rows, p->ldx) && tc_direct(p->dtype, p->w, p->out, p->ldw))
-    return 2.4 + fma / 6 < 5.7 + 0.18 * w;
-  return 2.4 + fma / 4.5 < 8 + 0.8 * w;
+  const bool f32 = p->dtype == PT_B200_F32;
+  const bool direct = tc_direct(p->dtype, p->x, p->rows, p->ldx) && tc_direct(p->dtype, p->w, p->out, p->ldw);
+  const double k = static_cast<double>(p->in), w = k * static_cast<double>(p->out) * 1e-6;
+  const double tasks = static_cast<double>((p->rows + kFewGroup - 1) / kFewGroup) * ((p->out + 1) / 2) * 1e-3;
+  const double fill = p->rows <= 1 ? 0.125 : p->rows <= 2 ? 0.25 : p->rows <= 4 ? 0.5 : 1.0;   // rows a task has
+  const double few = 2.4 + tasks * (0.7 + fill * k * (f32 ? 0.0014 : direct ? 0.0018 : 0.003));
+  const double start = 0.001 * (k < 1024 ? k : 1024);
+  return few < start + (f32 ? 7.6 + 2.4 * w : direct ? 4.6 + 0.18 * w : 5.7 + 0.9 * w);
 }
 
 }  // namespace
