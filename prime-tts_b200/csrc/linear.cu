@@ -158,7 +158,7 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
 
 // Whether a call takes the few-rows kernel: by the microseconds that both would take.  Its own follow
 // from its warps' tasks (two channels x eight rows), each a start and k; the tensor cores' from a start,
-// the weights and the first stages of k.  Fits to measurements (the tensor cores' in brackets, rows x
+// the first stages of k, the weights and x (in its planes, against a tile of 128 channels).  Fits to measurements (the tensor cores' in brackets, rows x
 // in x out):
 //   bf16  4 x 4096 x 1024 4.5 (6.8), 8 x 1024 x 1024 3.9 (5.9), 2 x 4096 x 4096 7.4 (8.8), 4 x 4096 x
 //         4096 10.5 (8.8), 64 x 192 x 768 5.7 (4.9), 1000 x 64 x 64 6.2 (4.5)
@@ -166,7 +166,7 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
 //         (5.9), 4 x 4001 x 4001 16.3 (21), 8 x 4001 x 4001 25.6 (21)
 //   fp32, which the tensor cores need in planes: 8 x 4096 x 4096 15.6 (48), 16 x 192 x 768 3.2 (8.7),
 //         128 x 768 x 192 5.3 (9.9), 2000 x 192 x 16 3.3 (9.4), 1000 x 192 x 192 14.1 (9.4)
-constexpr int kFewRows = 4096;
+constexpr int kFewRows = 1 << 18;
 bool few_rows(const pt_b200_linear_args *p) {
   if (p->rows > kFewRows) return false;
   const bool f32 = p->dtype == PT_B200_F32;
@@ -175,8 +175,8 @@ bool few_rows(const pt_b200_linear_args *p) {
   const double tasks = static_cast<double>((p->rows + kFewGroup - 1) / kFewGroup) * ((p->out + 1) / 2) * 1e-3;
   const double fill = p->rows <= 1 ? 0.125 : p->rows <= 2 ? 0.25 : p->rows <= 4 ? 0.5 : 1.0;   // rows a task has
   const double few = 2.4 + tasks * (0.7 + fill * k * (f32 ? 0.0014 : direct ? 0.0018 : 0.003));
-  const double start = 0.001 * (k < 1024 ? k : 1024);
-  return few < start + (f32 ? 7.6 + 2.4 * w : direct ? 4.6 + 0.18 * w : 5.7 + 0.9 * w);
+  const double start = 0.001 * (k < 1024 ? k : 1024), x = static_cast<double>(p->rows) * k * 1e-6;
+  return few < start + (f32 ? 7.6 + 2.4 * w + 4.0 * x : direct ? 4.6 + 0.18 * w + 0.6 * x : 5.7 + 0.9 * w + 1.4 * x);
 }
 
 }  // namespace
