@@ -20,13 +20,14 @@ struct FewArgs {
 };
 
 // ---- a few rows (single tokens): every weight is read once and used for all of them, so the call is
-// bound by the weights' bytes, and by its latency where they are few.  A warp takes two channels and a
-// share of k: it reads 16 bytes of each weight row and of each row of x (which stays in L1) per lane
-// and step, kAhead steps in flight with no branch between the loads, and adds up in fp32 FMAs.
-// Lanes, then the warps that share a channel's k, add up in a fixed order.  More rows than eight are
-// groups of eight, which read the weights again from L2.  1 x 4096 x 4096 bf16 5.8 us (5.8 TB/s), 8 x
-// 4096 x 4096 fp32 15.6 us; with twice as many warps, in two waves, 6.9 and 22.9.
-constexpr int kFewGroup = 8, kFewWarps = 8, kFewChans = 2, kFewFill = 8;
+// bound by the weights' bytes, and by its latency where they are few.  A warp takes two channels (four
+// where there are many rows, which halves what it reads of x) and a share of k: it reads 16 bytes of
+// each weight row and of each row of x (which stays in L1) per lane and step, kAhead steps in flight
+// with no branch between the loads, and adds up in fp32 FMAs.  Lanes, then the warps that share a
+// channel's k, add up in a fixed order.  More rows than eight are groups of eight, which read the
+// weights again from L2.  1 x 4096 x 4096 bf16 5.8 us (5.8 TB/s), 8 x 4096 x 4096 fp32 15.6 us; with
+// twice as many warps, in two waves, 6.9 and 22.9.
+constexpr int kFewGroup = 8, kFewWarps = 8, kFewFill = 8;
 
 // Sums of v[0 .. N) over the warp, by halves: N / 2 + N / 4 + ... exchanges, not 5 N.  Lane l holds
 // the sum of value (l / (32 / N)).
@@ -46,34 +47,35 @@ __device__ __forceinline__ float warp_sums(float (&v)[N], int lane) {
   return v[0];
 }
 
-template <class T, int R, bool VEC>
+template <class T, int R, int C, bool VEC>
 __global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const FewArgs a) {
   constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1, kAhead = VEC ? (R <= 2 ? 4 : R == 4 ? 2 : 1) : 4;
-  constexpr int kSums = kFewChans * R;
+  constexpr int kSums = C * R;
   using P = Pack<T, V>;
   __shared__ float part[kFewWarps][kSums];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int share = warp % a.shares, team = warp / a.shares;
   const int row0 = blockIdx.y * kFewGroup, rows = min(a.rows - row0, kFewGroup);
-  const int64_t chan = (static_cast<int64_t>(blockIdx.x) * (kFewWarps / a.shares) + team) * kFewChans;
+  const int64_t chan = (static_cast<int64_t>(blockIdx.x) * (kFewWarps / a.shares) + team) * C;
   float acc[kSums];
 #pragma unroll
   for (int i = 0; i < kSums; ++i) acc[i] = 0.0f;
   if (chan < a.out) {
     const int64_t step = static_cast<int64_t>(a.shares) * 32 * V;
     int64_t k = (share * 32 + lane) * V;
-    const T *w[kFewChans], *x[R];
-    w[0] = static_cast<const T *>(a.w) + chan * a.ldw + k;
-    w[1] = w[0] + (chan + 1 < a.out ? a.ldw : 0);          // (a last single channel twice)
+    const T *w[C], *x[R];
+#pragma unroll
+    for (int c = 0; c < C; ++c)   // (the last channel again in the place of one beyond)
+      w[c] = static_cast<const T *>(a.w) + (chan + c < a.out ? chan + c : a.out - 1) * a.ldw + k;
 #pragma unroll
     for (int r = 0; r < R; ++r) x[r] = static_cast<const T *>(a.x) + (row0 + (r < rows ? r : 0)) * a.ldx + k;
     auto steps = [&](auto count) {
       constexpr int A = decltype(count)::value;
-      P p[A][kFewChans], q[A][R];
+      P p[A][C], q[A][R];
 #pragma unroll
       for (int u = 0; u < A; ++u) {
 #pragma unroll
-        for (int c = 0; c < kFewChans; ++c) p[u][c] = *reinterpret_cast<const P *>(w[c] + u * step);
+        for (int c = 0; c < C; ++c) p[u][c] = *reinterpret_cast<const P *>(w[c] + u * step);
 #pragma unroll
         for (int r = 0; r < R; ++r) q[u][r] = *reinterpret_cast<const P *>(x[r] + u * step);
       }
@@ -84,10 +86,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const Few
 #pragma unroll
           for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int c = 0; c < kFewChans; ++c)
+            for (int c = 0; c < C; ++c)
               acc[c * R + r] = fmaf(to_f32(p[u][c].v[j]), to_f32(q[u][r].v[j]), acc[c * R + r]);
 #pragma unroll
-      for (int c = 0; c < kFewChans; ++c) w[c] += A * step;
+      for (int c = 0; c < C; ++c) w[c] += A * step;
 #pragma unroll
       for (int r = 0; r < R; ++r) x[r] += A * step;
       k += A * step;
@@ -114,15 +116,18 @@ int launch_few(const pt_b200_ops *h, const FewArgs &args, cudaStream_t st) {
   constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
   FewArgs a = args;
   // share a channel's k among warps until there are kFewFill on every SM, or a share is a single step
-  const int64_t teams = (a.out + kFewChans - 1) / kFewChans;
-  a.shares = 1;
   const int64_t groups = (a.rows + kFewGroup - 1) / kFewGroup;
+  // four channels a warp halve what it reads of x, where there is work for all warps even so
+  const bool four = a.rows > 4 && groups * ((a.out + 3) / 4) >= kFewFill * h->sms;
+  const int64_t teams = four ? (a.out + 3) / 4 : (a.out + 1) / 2;
+  a.shares = 1;
   while (a.shares < kFewWarps && teams * groups * a.shares < kFewFill * h->sms && a.in > a.shares * 32 * V) a.shares *= 2;
   const int64_t per_block = kFewWarps / a.shares;
   const unsigned blocks = static_cast<unsigned>((teams + per_block - 1) / per_block);
-  auto *kernel = a.rows == 1 ? linear_few_kernel<T, 1, VEC>
-                 : a.rows == 2 ? linear_few_kernel<T, 2, VEC>
-                 : a.rows <= 4 ? linear_few_kernel<T, 4, VEC> : linear_few_kernel<T, 8, VEC>;
+  auto *kernel = a.rows == 1 ? linear_few_kernel<T, 1, 2, VEC>
+                 : a.rows == 2 ? linear_few_kernel<T, 2, 2, VEC>
+                 : a.rows <= 4 ? linear_few_kernel<T, 4, 2, VEC>
+                 : four ? linear_few_kernel<T, 8, 4, VEC> : linear_few_kernel<T, 8, 2, VEC>;
   kernel<<<dim3(blocks, static_cast<unsigned>(groups)), kFewWarps * 32, 0, st>>>(a);
   PTB_CUDA(cudaGetLastError());
   count_launch();
@@ -165,7 +170,8 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
 //   not aligned, so that the tensor cores need copies: 128 x 101 x 201 4.4 (5.9), 500 x 101 x 201 10.1
 //         (5.9), 4 x 4001 x 4001 16.3 (21), 8 x 4001 x 4001 25.6 (21)
 //   fp32, which the tensor cores need in planes: 8 x 4096 x 4096 15.6 (48), 16 x 192 x 768 3.2 (8.7),
-//         128 x 768 x 192 5.3 (9.9), 2000 x 192 x 16 3.3 (9.4), 1000 x 192 x 192 14.1 (9.4)
+//         128 x 768 x 192 5.3 (9.9), 2000 x 192 x 16 3.3 (9.4), 700 x 192 x 192 7.4 (9.1), 7369 x
+//         2296 x 24 46 (68), 16064 x 347 x 40 (27)
 constexpr int kFewRows = 1 << 18;
 bool few_rows(const pt_b200_linear_args *p) {
   if (p->rows > kFewRows) return false;
@@ -174,7 +180,8 @@ bool few_rows(const pt_b200_linear_args *p) {
   const double k = static_cast<double>(p->in), w = k * static_cast<double>(p->out) * 1e-6;
   const double tasks = static_cast<double>((p->rows + kFewGroup - 1) / kFewGroup) * ((p->out + 1) / 2) * 1e-3;
   const double fill = p->rows <= 1 ? 0.125 : p->rows <= 2 ? 0.25 : p->rows <= 4 ? 0.5 : 1.0;   // rows a task has
-  const double few = 2.4 + tasks * (0.7 + fill * k * (f32 ? 0.0014 : direct ? 0.0018 : 0.003));
+  const double four = p->rows > 4 && tasks > 2.4 ? 0.7 : 1.0;   // many tasks, of four channels each
+  const double few = 2.4 + four * tasks * (0.7 + fill * k * (f32 ? 0.0014 : direct ? 0.0018 : 0.003));
   const double start = 0.001 * (k < 1024 ? k : 1024), x = static_cast<double>(p->rows) * k * 1e-6;
   return few < start + (f32 ? 7.6 + 2.4 * w + 4.0 * x : direct ? 4.6 + 0.18 * w + 0.6 * x : 5.7 + 0.9 * w + 1.4 * x);
 }
