@@ -7,7 +7,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -111,13 +111,17 @@ struct Call {
   }
 };
 
+// New tensors on like's device, from the allocator itself: the dispatcher's way to it takes as long.
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor &like) {
+  return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
+}
 // like's leading dimensions with `cols` columns.
 at::Tensor empty_rows(const at::Tensor &like, int64_t cols) {
   at::DimVector shape(like.sizes().begin(), like.sizes().end());
   shape.back() = cols;
-  return at::empty(shape, like.options());
+  return empty(shape, like.scalar_type(), like);
 }
-at::Tensor workspace(const at::Tensor &like, int64_t bytes) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
+at::Tensor workspace(const at::Tensor &like, int64_t bytes) { return empty({bytes}, at::kByte, like); }
 
 PyObject *wrap(at::Tensor t) { return t.defined() ? THPVariable_Wrap(std::move(t)) : Py_NewRef(Py_None); }
 PyObject *tuple3(at::Tensor a, at::Tensor b, at::Tensor c) {
@@ -195,11 +199,11 @@ PyObject *linear_backward(PyObject *const *o) {
     a.dx = dx.mutable_data_ptr();
   }
   if (need_dw) {
-    dw = at::empty({a.out, a.in}, dy.options());
+    dw = empty({a.out, a.in}, c.type, dy);
     a.dw = dw.mutable_data_ptr();
   }
   if (need_db) {
-    db = at::empty({a.out}, dy.options());
+    db = empty({a.out}, c.type, dy);
     a.db = db.mutable_data_ptr();
   }
   a.lddx = a.lddw = a.in;
@@ -228,10 +232,9 @@ PyObject *layer_norm(PyObject *const *o) {
   a.x = c.rows(x, "x", a.rows, a.cols, &a.ldx);
   a.gamma = c.vector(o[3], "gamma", c.type, a.cols);
   a.beta = c.vector(o[4], "beta", c.type, a.cols);
-  at::Tensor y = at::empty(x.sizes(), x.options());
+  at::Tensor y = empty(x.sizes(), c.type, x);
   const auto lead = x.sizes().slice(0, x.dim() - 1);
-  const auto f32 = x.options().dtype(at::kFloat);
-  at::Tensor mean = at::empty(lead, f32), rstd = at::empty(lead, f32);
+  at::Tensor mean = empty(lead, at::kFloat, x), rstd = empty(lead, at::kFloat, x);
   a.y = y.mutable_data_ptr();
   a.ldy = a.cols;
   a.mean = mean.mutable_data_ptr<float>();
@@ -259,16 +262,16 @@ PyObject *layer_norm_backward(PyObject *const *o) {
   a.rstd = static_cast<const float *>(c.vector(o[6], "rstd", at::kFloat, a.rows));
   at::Tensor dx, dgamma, dbeta, work;
   if (need_dx) {
-    dx = at::empty(dy.sizes(), dy.options());
+    dx = empty(dy.sizes(), c.type, dy);
     a.dx = dx.mutable_data_ptr();
     a.lddx = a.cols;
   }
   if (need_dg) {
-    dgamma = at::empty({a.cols}, dy.options());
+    dgamma = empty({a.cols}, c.type, dy);
     a.dgamma = dgamma.mutable_data_ptr();
   }
   if (need_db) {
-    dbeta = at::empty({a.cols}, dy.options());
+    dbeta = empty({a.cols}, c.type, dy);
     a.dbeta = dbeta.mutable_data_ptr();
   }
   if (need_dg || need_db) a.work_bytes = pt_b200_layer_norm_backward_work(c.h, a.rows, a.cols);
