@@ -433,6 +433,20 @@ def test_layer_norm(ops, dtype, rows, cols):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("cols", [100, 101, 1000, 1001, 3000, 6000, 10000])
+def test_layer_norm_backward_few_rows(ops, dtype, cols):
+    """Around the row counts where one block, a cluster of two to eight, and many blocks take over."""
+    g = _gen(cols)
+    x, dy = _randn(g, 130, cols).to(dtype), _randn(g, 130, cols).to(dtype)
+    gamma = _randn(g, cols).to(dtype)
+    _, mean, rstd = ops.layer_norm(x)
+    for rows in (1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129):
+        n = slice(0, rows)
+        got = ops.layer_norm_backward(dy[n], x[n], gamma, mean[n], rstd[n])
+        _check_norm_backward(got, dy[n], x[n], gamma, mean[n], rstd[n])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_layer_norm_backward_parts(ops, dtype):
     for rows, cols in ((50, 200), (20, 2048), (4, 17000)):
         g = _gen(cols)
@@ -579,11 +593,13 @@ def test_refusals_of_the_c_entries(ops):
                dict(ldy=20)):
         assert norm(**kw) == -1, kw
 
-    st = torch.zeros(6, device="cuda")
+    n = 300      # rows that need workspace (a few do without)
+    st, big, out = torch.zeros(n, device="cuda"), x.repeat(n // 6, 1), x.repeat(n // 6, 1)
+    assert L.pt_b200_layer_norm_backward_work(h, n, 24) > 0
 
     def norm_grad(**kw):
-        a = dict(dtype=1, res=0, rows=6, cols=24, dy=x.data_ptr(), x=x.data_ptr(), g=0, m=st.data_ptr(),
-                 rs=st.data_ptr(), dx=y.data_ptr(), dg=b.data_ptr(), db=0, lddy=24, ldx=24, lddx=24, work=0,
+        a = dict(dtype=1, res=0, rows=n, cols=24, dy=big.data_ptr(), x=big.data_ptr(), g=0, m=st.data_ptr(),
+                 rs=st.data_ptr(), dx=out.data_ptr(), dg=b.data_ptr(), db=0, lddy=24, ldx=24, lddx=24, work=0,
                  nbytes=0)
         a.update(kw)
         return L.pt_b200_layer_norm_backward(h, None, ops._NORM_GRAD.pack(*a.values()))
