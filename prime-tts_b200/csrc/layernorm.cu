@@ -21,8 +21,10 @@
 // read again instead of kept.
 //
 // Where rows are aligned a thread reads back only what it copied itself, with no barrier; where they
-// are not, the aligned 16-byte pieces that hold the row are copied (the bytes beside it are not
-// used) and every thread picks single elements.
+// are not, the aligned 16-byte pieces that hold the row are copied (the elements beside it are not
+// used, and none outside the tensor are read) and every thread picks single elements: 32768 x 1001 bf16
+// 44 us against 26 at 1024, which is instructions.  Two neighbours at a time, or whole pieces with the
+// row's ends masked, cost as many: 59 and 46 us.
 //
 // The weight gradients are column sums over all rows: each thread keeps its columns' sums over the
 // rows it walks; a block adds its rows' sums in shared memory and writes one row of partials, and a
@@ -103,6 +105,7 @@ struct NormArgs {
   void *y;                     // forward: y; backward: dx (may be null)
   float *mean, *rstd;          // forward: written (may be null); backward: read
   float *part;                 // backward: [blocks][2][cols] partial dgamma, dbeta (may be null)
+  const void *x_end, *dy_end;  // past the last row
   int64_t rows, cols, ldx, lddy, ldy;
   void *dgamma, *dbeta;        // backward, direct: written by the cluster itself (each may be null)
   bool direct;
@@ -123,16 +126,27 @@ struct Lay {
   static constexpr int kThreads = TPR > kBlock ? TPR : kBlock, kRows = kThreads / TPR;
   static constexpr int kRowBytes = TPR * kElems * static_cast<int>(sizeof(T));   // padded
   static constexpr int kSlot = kRows * (kRowBytes + (V == 1 ? 48 : 0)) * INPUTS;
-  // the blocks of an SM (launch bounds below) share 160 KB of it for their rings; more rows ahead
-  // than four changed nothing
-  static constexpr int kPerSm = INPUTS == 1 ? (kThreads == kBlock ? (V == 1 ? 3 : 4) : 2) : (kThreads == kBlock ? 2 : 1);
-  static constexpr int kFit = 160 * 1024 / kPerSm / kSlot;
+  // The blocks of an SM (launch bounds below) share 160 KB of it for their rings.  Forward, as many
+  // blocks as leave room for two slots each beside gamma and beta, or one where single elements are
+  // picked (8192 x 8192 fp16 46 us; with four blocks, which did not all fit, 65).  More rows ahead
+  // than four changed nothing.
+  static constexpr int room(int blocks) {
+    const int ring = 160 * 1024 / blocks, left = 224 * 1024 / blocks - 3 * 1024 - 2 * kRowBytes;
+    return INPUTS == 1 && left < ring ? left : ring;
+  }
+  static constexpr int per_sm(int most) {
+    return most > 1 && room(most) < (V == 1 ? 1 : 2) * kSlot ? per_sm(most - 1) : most;
+  }
+  static constexpr int kPerSm = INPUTS == 1 ? per_sm(kThreads == kBlock ? (V == 1 ? 3 : 4) : 2) : (kThreads == kBlock ? 2 : 1);
+  static constexpr int kFit = room(kPerSm) / kSlot;
   static constexpr int kDepth = kFit > 4 ? 4 : kFit < 1 ? 1 : kFit;
   static constexpr int kBytes = kSlot * kDepth;
   static constexpr int kParam = kRowBytes;                                       // gamma, or beta
 
-  // Starts the copies of row `row` (the TPR threads together); `at` is this input's part of a slot.
-  static __device__ __forceinline__ void fetch(uint32_t at, const T *row, int cols, int pitch, int t, int group) {
+  // Starts the copies of row `row` (the TPR threads together) of the tensor [begin, end); `at` is this
+  // input's part of a slot.
+  static __device__ __forceinline__ void fetch(uint32_t at, const T *row, const void *begin, const void *end,
+                                               int cols, int pitch, int t, int group) {
     if constexpr (V > 1) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -142,8 +156,19 @@ struct Lay {
     } else {
       const uintptr_t lo = reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15);
       const uintptr_t hi = reinterpret_cast<uintptr_t>(row + cols);
-      for (uintptr_t p = lo + t * 16; p < hi; p += TPR * 16)
-        copy16(at + group * pitch + static_cast<uint32_t>(p - lo), reinterpret_cast<const void *>(p));
+      const bool inside = lo >= reinterpret_cast<uintptr_t>(begin) && hi + 15 <= reinterpret_cast<uintptr_t>(end);
+      for (uintptr_t p = lo + t * 16; p < hi; p += TPR * 16) {
+        const uint32_t to = at + group * pitch + static_cast<uint32_t>(p - lo);
+        if (inside || (p >= reinterpret_cast<uintptr_t>(row) && p + 16 <= hi)) {
+          copy16(to, reinterpret_cast<const void *>(p));
+        } else {   // the tensor may begin or end inside this piece
+          const T *from = reinterpret_cast<const T *>(p);
+          T *slot = static_cast<T *>(__cvta_shared_to_generic(to));
+#pragma unroll
+          for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i)
+            if (from + i >= row && from + i < row + cols) slot[i] = from[i];
+        }
+      }
     }
   }
   static __device__ __forceinline__ int column(int unit, int t) {
@@ -210,7 +235,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_fwd_kernel(const 
   const int64_t xstep = step * a.ldx, ystep = step * a.ldy;
 #pragma unroll
   for (int d = 0; d < D - 1; ++d, ahead += step, xa += xstep) {
-    if (ahead < a.rows) L::fetch(at + d * L::kSlot, xa, cols, a.pitch, t, group);
+    if (ahead < a.rows) L::fetch(at + d * L::kSlot, xa, a.x, a.x_end, cols, a.pitch, t, group);
     copy_commit();
   }
   L::param(gamma, a.gamma, cols, 1.0f);
@@ -218,7 +243,7 @@ __global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_fwd_kernel(const 
   __syncthreads();
   int slot = 0, fill = D - 1;
   for (; r < a.rows; r += step, ahead += step, x += xstep, xa += xstep, y += ystep) {
-    if (ahead < a.rows) L::fetch(at + fill * L::kSlot, xa, cols, a.pitch, t, group);
+    if (ahead < a.rows) L::fetch(at + fill * L::kSlot, xa, a.x, a.x_end, cols, a.pitch, t, group);
     copy_commit();
     copy_wait<D - 1>();
     if constexpr (V == 1) row_sync<TPR>(group);
@@ -321,8 +346,8 @@ __global__ void __launch_bounds__(L::kThreads, L::kPerSm) norm_bwd_kernel(const 
   T *dx = static_cast<T *>(a.y) + r * a.ldy;
   const int64_t xstep = step * a.ldx, dstep = step * a.lddy, ystep = step * a.ldy;
   auto fetch = [&](int slot) {
-    L::fetch(at + slot * L::kSlot, xa, cols, a.pitch, t, group);
-    L::fetch(at + slot * L::kSlot + kHalf, da, cols, a.pitch, t, group);
+    L::fetch(at + slot * L::kSlot, xa, a.x, a.x_end, cols, a.pitch, t, group);
+    L::fetch(at + slot * L::kSlot + kHalf, da, a.dy, a.dy_end, cols, a.pitch, t, group);
   };
 #pragma unroll
   for (int d = 0; d < D - 1; ++d, ahead += step, xa += xstep, da += dstep) {
@@ -566,7 +591,8 @@ int64_t grid_rows(const pt_b200_ops *h, int64_t rows, int rows_per_block, int pe
 
 // fn.template operator()<TPR, V, N>() for the threads and elements of a row.  Few elements a thread
 // where there are too few rows to fill the GPU (`few`), where one row's latency counts: 64 x 4096 fp32
-// backward took 10.3 us with 32 elements and 7.7 with 16.  Backward, rows of up to 2048 keep 8 or 16
+// backward took 10.3 us with 32 elements and 7.7 with 16.  Single elements: 16 a thread, which need no
+// more than their registers (32768 x 1001 fp32 47 us, with 32 elements 64).  Backward, rows of up to 2048 keep 8 or 16
 // elements, whose sums leave room for more rows at once (8192 x 1000 fp16 16 us, with 32 elements 32).
 template <class T, bool VEC, bool FORWARD, class F>
 int pick(int64_t cols, bool few, F &&fn) {
@@ -576,7 +602,12 @@ int pick(int64_t cols, bool few, F &&fn) {
   if (cols <= 1024 && (few || !FORWARD)) return fn.template operator()<128, V, 8 / V>();
   if (cols <= 4096 && few) return fn.template operator()<512, V, 8 / V>();
   if (cols <= 8192 && (few || !FORWARD) && cols > 4096) return fn.template operator()<512, V, 16 / V>();
-  if constexpr (FORWARD) {
+  if constexpr (FORWARD && !VEC) {
+    if (cols <= 1024) return fn.template operator()<64, V, 16 / V>();
+    if (cols <= 2048) return fn.template operator()<128, V, 16 / V>();
+    if (cols <= 4096) return fn.template operator()<256, V, 16 / V>();
+    if (cols <= 8192) return fn.template operator()<512, V, 16 / V>();
+  } else if constexpr (FORWARD) {
     if (cols <= 1024) return fn.template operator()<32, V, 32 / V>();
     if (cols <= 2048) return fn.template operator()<64, V, 32 / V>();
     if (cols <= 8192 && cols > 4096) return fn.template operator()<256, V, 32 / V>();
@@ -703,6 +734,7 @@ extern "C" int pt_b200_layer_norm(pt_b200_ops *h, void *stream, const pt_b200_no
   a.ldx = p->ldx;
   a.ldy = p->ldy;
   a.eps = p->eps;
+  a.x_end = static_cast<const char *>(p->x) + ((p->rows - 1) * p->ldx + p->cols) * eb;
   a.pitch = static_cast<int>(round_up(p->cols * eb, 16) + 32);
   const int v = 16 / eb;
   const bool vec = p->cols % v == 0 && (p->rows == 1 || (p->ldx % v == 0 && p->ldy % v == 0)) &&
@@ -763,7 +795,9 @@ extern "C" int pt_b200_layer_norm_backward(pt_b200_ops *h, void *stream,
   a.cols = p->cols;
   a.ldx = p->ldx;
   a.lddy = p->lddy;
+  a.dy_end = static_cast<const char *>(p->dy) + ((p->rows - 1) * p->lddy + p->cols) * eb;
   a.ldy = p->lddx;
+  a.x_end = static_cast<const char *>(p->x) + ((p->rows - 1) * p->ldx + p->cols) * eb;
   a.pitch = static_cast<int>(round_up(p->cols * eb, 16) + 32);
   const int v = 16 / eb;
   const bool vec = p->cols % v == 0 &&

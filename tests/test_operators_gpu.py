@@ -447,6 +447,24 @@ def test_layer_norm_backward_few_rows(ops, dtype, cols):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("cols", [3, 37, 512, 1003])
+def test_layer_norm_begins_anywhere(ops, dtype, cols):
+    """Tensors that begin, and whose rows lie, at any element of a 16-byte piece."""
+    g = _gen(cols)
+    rows, n = 41, 41 * (cols + 5) + 9
+    fx, fd = _randn(g, n).to(dtype), _randn(g, n).to(dtype)
+    gamma = _randn(g, cols).to(dtype)
+    for begin in range(9):
+        for pad in (0, 1, 5):
+            ld = cols + pad
+            x = fx[begin:begin + rows * ld].view(rows, ld)[:, :cols]
+            dy = fd[8 - begin:8 - begin + rows * ld].view(rows, ld)[:, :cols]
+            y, mean, rstd = ops.layer_norm(x, gamma, eps=EPS)
+            _check_norm(y, mean, rstd, x, gamma, None)
+            _check_norm_backward(ops.layer_norm_backward(dy, x, gamma, mean, rstd), dy, x, gamma, mean, rstd)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_layer_norm_backward_parts(ops, dtype):
     for rows, cols in ((50, 200), (20, 2048), (4, 17000)):
         g = _gen(cols)
