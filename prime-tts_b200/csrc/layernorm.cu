@@ -593,7 +593,8 @@ int64_t grid_rows(const pt_b200_ops *h, int64_t rows, int rows_per_block, int pe
 // where there are too few rows to fill the GPU (`few`), where one row's latency counts: 64 x 4096 fp32
 // backward took 10.3 us with 32 elements and 7.7 with 16.  Single elements: 16 a thread, which need no
 // more than their registers (32768 x 1001 fp32 47 us, with 32 elements 64).  Backward, rows of up to 2048 keep 8 or 16
-// elements, whose sums leave room for more rows at once (8192 x 1000 fp16 16 us, with 32 elements 32).
+// elements, whose sums leave room for more rows at once (8192 x 1000 fp16 16 us, with 32 elements 32);
+// rows of up to 8192 take 32 on 256 threads, two blocks an SM (4000 x 6144 bf16 40 us, with 16 on 512 46).
 template <class T, bool VEC, bool FORWARD, class F>
 int pick(int64_t cols, bool few, F &&fn) {
   constexpr int V = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
@@ -601,7 +602,7 @@ int pick(int64_t cols, bool few, F &&fn) {
   if (cols <= 512) return fn.template operator()<32, V, 16 / V>();
   if (cols <= 1024 && (few || !FORWARD)) return fn.template operator()<128, V, 8 / V>();
   if (cols <= 4096 && few) return fn.template operator()<512, V, 8 / V>();
-  if (cols <= 8192 && (few || !FORWARD) && cols > 4096) return fn.template operator()<512, V, 16 / V>();
+  if (cols <= 8192 && few && cols > 4096) return fn.template operator()<512, V, 16 / V>();
   if constexpr (FORWARD && !VEC) {
     if (cols <= 1024) return fn.template operator()<64, V, 16 / V>();
     if (cols <= 2048) return fn.template operator()<128, V, 16 / V>();
@@ -613,6 +614,7 @@ int pick(int64_t cols, bool few, F &&fn) {
     if (cols <= 8192 && cols > 4096) return fn.template operator()<256, V, 32 / V>();
   } else {
     if (cols <= 2048) return fn.template operator()<128, V, 16 / V>();
+    if (cols <= 8192 && cols > 4096) return fn.template operator()<256, V, 32 / V>();
   }
   if (cols <= 4096) return fn.template operator()<128, V, 32 / V>();
   return fn.template operator()<512, V, 32 / V>();
@@ -627,7 +629,7 @@ int rows_per_block(const pt_b200_ops *h, int64_t rows, int64_t cols) {
 int bwd_blocks(const pt_b200_ops *h, int64_t rows, int64_t cols) {
   if (cols > kMaxRegCols) return static_cast<int>(rows < 8 * 64 ? (rows + 7) / 8 : 64);
   return static_cast<int>(
-      grid_rows(h, rows, rows_per_block(h, rows, cols), cols <= 1024 || (cols <= 4096 && !few_rows(h, rows)) ? 2 : 1));
+      grid_rows(h, rows, rows_per_block(h, rows, cols), cols <= 1024 || (cols <= 8192 && !few_rows(h, rows)) ? 2 : 1));
 }
 // Blocks of the cluster that does a few rows alone (two turns each), or 0.
 int direct_blocks(const pt_b200_ops *h, int64_t rows, int64_t cols) {
