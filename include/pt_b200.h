@@ -500,8 +500,8 @@ PT_B200_API int pt_b200_layer_norm(pt_b200_ops *h, void *stream, const pt_b200_n
 /* With g = dy * gamma and xhat = (x - mean) * rstd: dx = rstd * (g - mean(g) - xhat * mean(g *
  * xhat)); dgamma = sum over rows of dy * xhat; dbeta = sum over rows of dy.  mean and rstd are
  * the forward pass's.  dx, dgamma and dbeta may each be NULL; dx may be dy itself (with its
- * stride).  Workspace is needed for dgamma / dbeta of more than a few rows only.  rows = 0 writes zeros to dgamma and
- * dbeta. */
+ * stride).  Workspace is needed for dgamma / dbeta of more than a few rows only.  rows = 0 writes
+ * zeros to dgamma and dbeta. */
 typedef struct {
   int32_t dtype, reserved;
   int64_t rows, cols;

@@ -3,7 +3,9 @@
 //   pre = x W^T + b;  y = act(pre) + r
 //   dpre = dy * act'(pre);  dx = dpre W;  dW = dpre^T x;  db = sum over rows of dpre
 //
-// The three products run on the tensor cores (linear_tc.cu).
+// The three products run on the tensor cores (linear_tc.cu); x W^T of a few rows, and of fp32 rows against
+// a few channels, in kernels of their own.
+#include <algorithm>
 #include <type_traits>
 
 #include "linear_tc.cuh"
@@ -134,6 +136,123 @@ int launch_few(const pt_b200_ops *h, const FewArgs &args, cudaStream_t st) {
   return 0;
 }
 
+// ---- fp32, many rows and up to 32 channels: the tensor cores would need planes of all of x, which is
+// most of what such a call moves, for products that are a fraction of it.  Here x and the weights go
+// through a ring of kNarrowStages steps of 64 of k in shared memory (asynchronous copies, zeros beyond
+// the matrices) and the sums are packed fp32 FMAs over pairs of k: a block has 64 rows and all
+// channels, a thread four rows (16 apart) and C channels (8 apart), and two groups of threads half of
+// each step's k.  Pieces of 16 bytes sit at their place XOR their row, so that neither reads collide.
+// Two blocks an SM keep the FMA pipe half busy, next to shared memory's reads.  16384 x 4096 x 32
+// 131 us (few rows 238), 15434 x 1592 x 25 55 (81), 16000 x 1592 x 4 30 (73), 16000 x 100 x 20 7.7 (17);
+// eight rows a thread and a quarter of k, which reads less: 133, 57, 28, 9.4.
+constexpr int kNarrowRows = 64, kNarrowK = 64, kNarrowStages = 3, kNarrowBlock = 256, kNarrowMost = 32;
+
+template <int C, bool VEC>
+__global__ void __launch_bounds__(kNarrowBlock, 2) linear_narrow_kernel(const FewArgs a) {
+  constexpr int kStage = (kNarrowRows + 8 * C) * kNarrowK;   // floats
+  constexpr int kXCopies = kNarrowRows / 16, kWCopies = (8 * C + 15) / 16;
+  extern __shared__ __align__(128) float ring_f[];           // [stages][64 rows of x, 8 C of w][64 of k]
+  const int tid = threadIdx.x, group = tid >> 7, tx = tid & 7, ty = tid >> 3 & 15;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kNarrowRows;
+  // copies: piece `piece` of rows line, line + 16, ...
+  const int piece = tid & 15, line = tid >> 4;
+  const uint32_t to = smem_u32(ring_f) + (line * kNarrowK + ((piece ^ (line & 7)) << 2)) * 4;
+  const float *x = static_cast<const float *>(a.x), *w = static_cast<const float *>(a.w);
+  const int steps = static_cast<int>((a.in + kNarrowK - 1) / kNarrowK);
+  auto copy = [&](uint32_t dst, const float *base, int64_t row, int64_t rows, int64_t ld, int64_t k) {
+    if constexpr (VEC) {
+      const bool in = row < rows && k < a.in;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? base + row * ld + k : base),
+                   "r"(in ? 16 : 0)
+                   : "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = row < rows && k + i < a.in;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + 4 * i),
+                     "l"(in ? base + row * ld + k + i : base), "r"(in ? 4 : 0)
+                     : "memory");
+      }
+    }
+  };
+  auto fetch = [&](int step) {
+    if (step < steps) {
+      const uint32_t at = to + step % kNarrowStages * (kStage * 4);
+      const int64_t k = static_cast<int64_t>(step) * kNarrowK + piece * 4;
+#pragma unroll
+      for (int i = 0; i < kXCopies; ++i) copy(at + i * 16 * kNarrowK * 4, x, row0 + line + 16 * i, a.rows, a.ldx, k);
+#pragma unroll
+      for (int i = 0; i < kWCopies; ++i)
+        if (line + 16 * i < 8 * C)
+          copy(at + (kNarrowRows + i * 16) * kNarrowK * 4, w, line + 16 * i, a.out, a.ldw, k);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  float2 acc[4][C];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < C; ++j) acc[i][j] = both(0.0f);
+#pragma unroll
+  for (int s = 0; s < kNarrowStages - 1; ++s) fetch(s);
+  for (int s = 0; s < steps; ++s) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kNarrowStages - 2) : "memory");
+    __syncthreads();   // step s has arrived, and the slot of step s - 1 has been read
+    fetch(s + kNarrowStages - 1);
+    const float *xs = ring_f + s % kNarrowStages * kStage, *ws = xs + kNarrowRows * kNarrowK;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const int at = group * 8 + c;
+      float4 p[4], q[C];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        p[i] = *reinterpret_cast<const float4 *>(xs + (ty + 16 * i) * kNarrowK + ((at ^ (ty & 7)) << 2));
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+        q[j] = *reinterpret_cast<const float4 *>(ws + (tx + 8 * j) * kNarrowK + ((at ^ tx) << 2));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          acc[i][j] = fma2(make_float2(p[i].x, p[i].y), make_float2(q[j].x, q[j].y), acc[i][j]);
+          acc[i][j] = fma2(make_float2(p[i].z, p[i].w), make_float2(q[j].z, q[j].w), acc[i][j]);
+        }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float *other = ring_f + (tid & 127);   // the second group's sums, [4 C][128]
+  if (group == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < C; ++j) other[(i * C + j) * 128] = acc[i][j].x + acc[i][j].y;
+  }
+  __syncthreads();
+  if (group == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int64_t row = row0 + ty + 16 * i;
+        const int chan = tx + 8 * j;
+        if (row < a.rows && chan < a.out)
+          linear_store<float>(a.e, row, chan, acc[i][j].x + acc[i][j].y + other[(i * C + j) * 128]);
+      }
+  }
+}
+
+template <int C>
+int launch_narrow(const FewArgs &a, bool vec, cudaStream_t st) {
+  constexpr int kBytes = kNarrowStages * (kNarrowRows + 8 * C) * kNarrowK * 4;
+  auto *kernel = vec ? linear_narrow_kernel<C, true> : linear_narrow_kernel<C, false>;
+  PTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  kernel<<<static_cast<unsigned>((a.rows + kNarrowRows - 1) / kNarrowRows), kNarrowBlock, kBytes, st>>>(a);
+  PTB_CUDA(cudaGetLastError());
+  count_launch();
+  return 0;
+}
+
 // An operand: the tensor itself where the tensor cores can read it, else its planes in the
 // workspace, which a pass of `jobs` fills.
 int64_t operand_bytes(int dtype, const void *p, int64_t rows, int64_t cols, int64_t ld) {
@@ -161,7 +280,7 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
          n_out < (int64_t(1) << 30);
 }
 
-// Whether a call takes the few-rows kernel: by the microseconds that both would take.  Its own follow
+// The kernel that a call takes: by the microseconds that each would take.  Its own follow
 // from its warps' tasks (two channels x eight rows), each a start and k; the tensor cores' from a start,
 // the first stages of k, the weights and x (in its planes, against a tile of 128 channels).  Fits to measurements (the tensor cores' in brackets, rows x
 // in x out):
@@ -172,25 +291,45 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
 //   fp32, which the tensor cores need in planes: 8 x 4096 x 4096 15.6 (48), 16 x 192 x 768 3.2 (8.7),
 //         128 x 768 x 192 5.3 (9.9), 2000 x 192 x 16 3.3 (9.4), 700 x 192 x 192 7.4 (9.1), 7369 x
 //         2296 x 24 46 (68), 16064 x 347 x 40 (27)
+// The few-rows kernel waits for an x that does not stay in L2.  The narrow one takes a start and, for each
+// 64 rows on an SM, steps of k: 1000 x 4096 x 32 73 us (few rows 15.5), 4000 x 1024 x 16 15 (10.5), 2000 x
+// 192 x 16 5.5 (3.3), 7369 x 2296 x 24 45 (46), 19434 x 192 x 32 13.9 (tensor cores 19.9).
+// Whether x and w can be read 16 bytes at a time.
+bool copies_whole(const pt_b200_linear_args *p) {
+  const int v = 16 / dtype_bytes(p->dtype);
+  auto aligned = [&](const void *q, int64_t rows, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows == 1 || ld % v == 0);
+  };
+  return p->in % v == 0 && aligned(p->x, p->rows, p->ldx) && aligned(p->w, p->out, p->ldw);
+}
+enum class Way { kTensor, kFew, kNarrow };
 constexpr int kFewRows = 1 << 18;
-bool few_rows(const pt_b200_linear_args *p) {
-  if (p->rows > kFewRows) return false;
+Way way(const pt_b200_ops *h, const pt_b200_linear_args *p) {
   const bool f32 = p->dtype == PT_B200_F32;
   const bool direct = tc_direct(p->dtype, p->x, p->rows, p->ldx) && tc_direct(p->dtype, p->w, p->out, p->ldw);
   const double k = static_cast<double>(p->in), w = k * static_cast<double>(p->out) * 1e-6;
   const double tasks = static_cast<double>((p->rows + kFewGroup - 1) / kFewGroup) * ((p->out + 1) / 2) * 1e-3;
   const double fill = p->rows <= 1 ? 0.125 : p->rows <= 2 ? 0.25 : p->rows <= 4 ? 0.5 : 1.0;   // rows a task has
   const double four = p->rows > 4 && tasks > 2.4 ? 0.7 : 1.0;   // many tasks, of four channels each
-  const double few = 2.4 + four * tasks * (0.7 + fill * k * (f32 ? 0.0014 : direct ? 0.0018 : 0.003));
   const double start = 0.001 * (k < 1024 ? k : 1024), x = static_cast<double>(p->rows) * k * 1e-6;
-  return few < start + (f32 ? 7.6 + 2.4 * w + 4.0 * x : direct ? 4.6 + 0.18 * w + 0.6 * x : 5.7 + 0.9 * w + 1.4 * x);
+  const double wait = f32 && x > 8 ? 1.6 * (x - 8) : 0.0;
+  const double few = 2.4 + wait + four * tasks * (0.7 + fill * k * (f32 ? 0.0014 : direct ? 0.0018 : 0.003));
+  const double tensor =
+      start + (f32 ? 7.6 + 2.4 * w + 4.0 * x : direct ? 4.6 + 0.18 * w + 0.6 * x : 5.7 + 0.9 * w + 1.4 * x);
+  if (f32 && p->out <= kNarrowMost) {
+    const int64_t blocks = (p->rows + kNarrowRows - 1) / kNarrowRows, steps = (p->in + kNarrowK - 1) / kNarrowK;
+    const double each = (p->out <= 8 ? 0.55 : p->out <= 16 ? 0.75 : 1.1) * (copies_whole(p) ? 1.0 : 1.35);
+    if (3.0 + each * static_cast<double>(steps * ((blocks + h->sms - 1) / h->sms)) < std::min(few, tensor))
+      return Way::kNarrow;
+  }
+  return p->rows <= kFewRows && few < tensor ? Way::kFew : Way::kTensor;
 }
 
 }  // namespace
 
 extern "C" int64_t pt_b200_linear_work(const pt_b200_ops *h, const pt_b200_linear_args *p) {
   if (!h || !p || !sizes_ok(p->rows, p->in, p->out) || p->rows == 0) return 0;
-  if (few_rows(p)) return 0;
+  if (way(h, p) != Way::kTensor) return 0;
   return operand_bytes(p->dtype, p->x, p->rows, p->in, p->ldx) +
          operand_bytes(p->dtype, p->w, p->out, p->in, p->ldw);
 }
@@ -215,13 +354,14 @@ extern "C" int pt_b200_linear(pt_b200_ops *h, void *stream, const pt_b200_linear
   PTB_REQUIRE(on.ok, "pt_b200_linear: device %d cannot be used", h->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const LinearEpi epi{p->bias, p->residual, p->y, p->pre, p->ldr, p->ldy, p->ldp, p->act, p->slope};
-  if (few_rows(p)) {
+  const Way by = way(h, p);
+  if (by != Way::kTensor) {
     const FewArgs a{p->x, p->w, p->in, p->out, p->ldx, p->ldw, static_cast<int>(p->rows), 1, epi};
-    const int v = 16 / eb;
-    auto aligned = [&](const void *q, int64_t rows, int64_t ld) {
-      return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows == 1 || ld % v == 0);
-    };
-    const bool vec = p->in % v == 0 && aligned(p->x, p->rows, p->ldx) && aligned(p->w, p->out, p->ldw);
+    const bool vec = copies_whole(p);
+    if (by == Way::kNarrow)
+      return p->out <= 8    ? launch_narrow<1>(a, vec, st)
+             : p->out <= 16 ? launch_narrow<2>(a, vec, st)
+                            : launch_narrow<4>(a, vec, st);
     return with_dtype(p->dtype, [&](auto *z) -> int {
       using T = std::remove_pointer_t<decltype(z)>;
       return vec ? launch_few<T, true>(h, a, st) : launch_few<T, false>(h, a, st);

@@ -129,6 +129,18 @@ def test_linear(ops, dtype, rows, n_in, n_out):
     _check_linear(ops.linear(x, w), x, w, None, None, "none")
 
 
+@pytest.mark.parametrize("rows,n_in,n_out", [(40000, 64, 1), (40001, 67, 7), (30000, 3, 8), (19434, 100, 9),
+                                             (19433, 129, 16), (19434, 192, 17), (9501, 130, 25), (16385, 256, 32),
+                                             (9500, 1000, 4)])
+def test_linear_many_rows_few_channels(ops, rows, n_in, n_out):
+    x, w, b, r = _linear_case(rows + n_in, torch.float32, rows, n_in, n_out)
+    y, pre = ops.linear(x, w, b, residual=r, act="silu", save_pre=True)
+    _check_linear(y, x, w, b, r, "silu", pre)
+    x, w, _, _ = _linear_case(rows + n_in, torch.float32, rows, n_in + 3, n_out)   # rows that are not aligned
+    x, w = x[:, 1:-2], w[:, 2:-1]
+    _check_linear(ops.linear(x, w), x, w, None, None, "none")
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("act", ["none", "leaky", "relu", "gelu", "silu"])
 def test_linear_activations(ops, dtype, act):
