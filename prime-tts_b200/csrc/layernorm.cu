@@ -809,13 +809,13 @@ extern "C" int pt_b200_layer_norm_backward(pt_b200_ops *h, void *stream,
     using T = std::remove_pointer_t<decltype(z)>;
     int parts = bwd_blocks(h, a.rows, a.cols);
     if (a.cols > kMaxRegCols) {
-      if (a.y && launch_rows(norm_bwd_wide_kernel<T>, grid_rows(h, a.rows, 1, 8), kBlock, 0, a, st)) return -1;
-      if (sums) {
+      if (sums) {   // before dx, which may lie over dy
         norm_cols_wide_kernel<T>
             <<<dim3(static_cast<unsigned>((a.cols + 31) / 32), parts), kBlock, 0, st>>>(a);
         PTB_CUDA(cudaGetLastError());
         count_launch();
       }
+      if (a.y && launch_rows(norm_bwd_wide_kernel<T>, grid_rows(h, a.rows, 1, 8), kBlock, 0, a, st)) return -1;
     } else if (vec ? pick<T, true, false>(a.cols, few_rows(h, a.rows), BwdLaunch<T>{h, a, st})
                    : pick<T, false, false>(a.cols, few_rows(h, a.rows), BwdLaunch<T>{h, a, st})) {
       return -1;
