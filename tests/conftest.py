@@ -28,7 +28,7 @@ def reference_dir():
                 d = json.load(f).get("reference_path")
         except Exception:
             d = None
-    return d if d and os.path.isdir(d) else None
+    return d if d and os.path.isdir(os.path.join(d, "runtime", "v21", "src")) else None
 
 
 def pytest_configure(config):
