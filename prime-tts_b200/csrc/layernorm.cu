@@ -718,7 +718,9 @@ extern "C" int pt_b200_layer_norm(pt_b200_ops *h, void *stream, const pt_b200_no
               (long long)p->rows, (long long)p->cols);
   const int eb = dtype_bytes(p->dtype);
   PTB_REQUIRE(rows_ok(p->x, p->rows, p->cols, p->ldx, eb) && rows_ok(p->y, p->rows, p->cols, p->ldy, eb),
-              "pt_b200_layer_norm: x and y need a pointer and a row stride of at least cols");
+              "pt_b200_layer_norm: x and y need an aligned pointer and a row stride of at least cols");
+  PTB_REQUIRE(element_ok(p->gamma, eb) && element_ok(p->beta, eb) && element_ok(p->mean, 4) && element_ok(p->rstd, 4),
+              "pt_b200_layer_norm: gamma, beta, mean or rstd is not aligned to its elements");
   PTB_REQUIRE(p->eps >= 0.0f, "pt_b200_layer_norm: eps must not be negative");
   if (p->rows == 0) return 0;
   DeviceScope on(h->device);
@@ -766,7 +768,10 @@ extern "C" int pt_b200_layer_norm_backward(pt_b200_ops *h, void *stream,
   const int eb = dtype_bytes(p->dtype);
   PTB_REQUIRE(rows_ok(p->x, p->rows, p->cols, p->ldx, eb) && rows_ok(p->dy, p->rows, p->cols, p->lddy, eb) &&
                   (!p->dx || rows_ok(p->dx, p->rows, p->cols, p->lddx, eb)),
-              "pt_b200_layer_norm_backward: x, dy and dx need a pointer and a row stride of at least cols");
+              "pt_b200_layer_norm_backward: x, dy and dx need an aligned pointer and a row stride of at least cols");
+  PTB_REQUIRE(element_ok(p->gamma, eb) && element_ok(p->mean, 4) && element_ok(p->rstd, 4) &&
+                  element_ok(p->dgamma, eb) && element_ok(p->dbeta, eb),
+              "pt_b200_layer_norm_backward: gamma, mean, rstd, dgamma or dbeta is not aligned to its elements");
   PTB_REQUIRE(p->rows == 0 || (p->mean && p->rstd), "pt_b200_layer_norm_backward: mean and rstd are needed");
   PTB_REQUIRE(p->rows == 0 || p->dx || p->dgamma || p->dbeta, "pt_b200_layer_norm_backward: nothing to compute");
   DeviceScope on(h->device);

@@ -346,9 +346,11 @@ extern "C" int pt_b200_linear(pt_b200_ops *h, void *stream, const pt_b200_linear
   const int eb = dtype_bytes(p->dtype);
   PTB_REQUIRE(rows_ok(p->x, p->rows, p->in, p->ldx, eb) && rows_ok(p->w, p->out, p->in, p->ldw, eb) &&
                   rows_ok(p->y, p->rows, p->out, p->ldy, eb),
-              "pt_b200_linear: x, w and y need a pointer and a row stride of at least their columns");
+              "pt_b200_linear: x, w and y need an aligned pointer and a row stride of at least their columns");
   PTB_REQUIRE((!p->residual || p->ldr >= p->out) && (!p->pre || p->ldp >= p->out),
               "pt_b200_linear: residual and pre need a row stride of at least out");
+  PTB_REQUIRE(element_ok(p->bias, eb) && element_ok(p->residual, eb) && element_ok(p->pre, eb),
+              "pt_b200_linear: bias, residual or pre is not aligned to its elements");
   if (p->rows == 0) return 0;
   DeviceScope on(h->device);
   PTB_REQUIRE(on.ok, "pt_b200_linear: device %d cannot be used", h->device);
@@ -414,11 +416,13 @@ extern "C" int pt_b200_linear_backward(pt_b200_ops *h, void *stream, const pt_b2
   PTB_REQUIRE(p->dx || p->dw || p->db, "pt_b200_linear_backward: nothing to compute");
   PTB_REQUIRE(rows_ok(p->dy, p->rows, p->out, p->lddy, eb) &&
                   (!acts || rows_ok(p->pre, p->rows, p->out, p->ldp, eb)),
-              "pt_b200_linear_backward: dy (and pre where there is an activation) needs a pointer and a "
+              "pt_b200_linear_backward: dy (and pre where there is an activation) needs an aligned pointer and a "
               "row stride of at least out");
   PTB_REQUIRE((!p->dx || (rows_ok(p->w, p->out, p->in, p->ldw, eb) && p->lddx >= p->in)) &&
                   (!p->dw || (rows_ok(p->x, p->rows, p->in, p->ldx, eb) && p->lddw >= p->in)),
               "pt_b200_linear_backward: dx needs w and dw needs x, with row strides of at least in");
+  PTB_REQUIRE(element_ok(p->dx, eb) && element_ok(p->dw, eb) && element_ok(p->db, eb),
+              "pt_b200_linear_backward: dx, dw or db is not aligned to its elements");
   DeviceScope on(h->device);
   PTB_REQUIRE(on.ok, "pt_b200_linear_backward: device %d cannot be used", h->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -202,9 +202,11 @@ struct ColumnSums {
 template <class T>
 int reduce_columns(const float *part, int parts, int64_t n, T *out, cudaStream_t st);
 
-// ---- argument checks shared by the entry points
+// ---- argument checks shared by the entry points: a kernel reads and writes whole elements, so a
+// pointer that is not aligned to its element would be an address fault on the device
+inline bool element_ok(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 inline bool rows_ok(const void *p, int64_t rows, int64_t cols, int64_t ld, int bytes) {
-  return rows == 0 || (p && ld >= cols && (reinterpret_cast<uintptr_t>(p) % bytes) == 0);
+  return rows == 0 || (p && ld >= cols && element_ok(p, bytes));
 }
 
 }  // namespace ptb
