@@ -77,10 +77,18 @@ struct Call {
   bool here(const at::Tensor &t) const { return t.is_cuda() && t.get_device() == device; }
   cudaStream_t stream() const { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
 
+  // Tensors whose values are not what lies in memory: torch keeps a pending minus sign (x.conj().imag), or
+  // no memory at all for zeros.
+  static void in_memory(const at::Tensor &t, const char *name) {
+    if (t.is_neg()) refuse(name, ": is a negated view, whose sign is not in memory (resolve_neg() puts it there)");
+    if (t._is_zerotensor()) refuse(name, ": is a tensor of zeros without memory (clone() gives it some)");
+  }
+
   // A [..., cols] tensor seen as [rows][cols] with one stride for its rows.
   const void *rows(const at::Tensor &t, const char *name, int64_t n, int64_t cols, int64_t *ld) const {
     if (t.scalar_type() != type || !here(t) || t.dim() == 0 || t.size(-1) != cols || t.numel() != n * cols)
       refuse(name, ": needs ", n, " rows of ", cols, " ", type_name(type), " on cuda:", device, ", got ", describe(t));
+    in_memory(t, name);
     *ld = cols;
     if (t.is_contiguous()) return t.const_data_ptr();
     int64_t stride = 0, step = 0;
@@ -107,6 +115,7 @@ struct Call {
     const at::Tensor &t = tensor(o, name);
     if (t.scalar_type() != want || !here(t) || t.numel() != n || !t.is_contiguous())
       refuse(name, ": needs ", n, " contiguous ", type_name(want), " on cuda:", device, ", got ", describe(t));
+    in_memory(t, name);
     return t.const_data_ptr();
   }
 };

@@ -45,3 +45,26 @@ def test_norm_gradient_over_dy(ops, dtype, rows, cols):
         need)) == 0
     for got, ref in zip((dx, dgamma, dbeta), want):
         assert torch.equal(got, ref)
+
+
+def test_tensors_whose_values_are_not_in_memory(ops):
+    """A negated view and a zero tensor without memory are refused, in every place of every call."""
+    z = torch.view_as_complex(_randn(1, 6, 8, 2)).conj().imag[:, :1]    # one column, a stride of 16
+    assert z.is_neg() and z.stride(0) == 16
+    launches = pt_b200.kernel_launches()
+    with pytest.raises(pt_b200.PtB200Error, match="x: is a negated view"):
+        ops.linear(z, _randn(2, 4, 1))
+    m, v, s = _randn(3, 6, 24), _randn(4, 24), _randn(5, 6)
+    w = _randn(6, 24, 24)
+    calls = [(ops.linear, dict(x=m, w=w, bias=v, residual=m)),
+             (ops.linear_backward, dict(dy=m, x=m, w=w, pre=m, act="gelu")),
+             (ops.layer_norm, dict(x=m, gamma=v, beta=v)),
+             (ops.layer_norm_backward, dict(dy=m, x=m, gamma=v, mean=s, rstd=s))]
+    for call, args in calls:
+        for name, t in args.items():
+            if isinstance(t, torch.Tensor):
+                with pytest.raises(pt_b200.PtB200Error, match=f"{name}: is a negated view"):
+                    call(**{**args, name: torch._neg_view(t)})
+                with pytest.raises(pt_b200.PtB200Error, match=f"{name}: is a tensor of zeros without memory"):
+                    call(**{**args, name: torch._efficientzerotensor(t.shape, device="cuda")})
+    assert pt_b200.kernel_launches() == launches
