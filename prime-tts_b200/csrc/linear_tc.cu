@@ -15,12 +15,18 @@
 //   dx        A = W   [out][in] MN-major   B = dpre [rows][out] K-major
 //   dW        A = x   [rows][in] MN-major  B = dpre [rows][out] MN-major
 //
-// bf16 and fp16 run as they are (one plane).  An fp32 operand is the sum of three bf16 planes
-// (3 x 8 significant bits; the differences are exact), and the product is the six plane products
-// that reach 2^-24 of it: a3 b1, a1 b3, a2 b2, a2 b1, a1 b2, a1 b1, smallest first.  The tensor
-// core's fp32 accumulator truncates each addition, which would bias a long sum, so every chunk of
-// k starts a new accumulator and the epilogue warps add the chunks in registers, rounding to
+// The tensor core's fp32 accumulator truncates each addition, which biases a long sum: fp16 gradients of
+// weights over 262144 rows of one sign came out 2.1e-4 too small, over 4194304 rows 3.3e-3.  So an
+// accumulator takes a chunk of k, and the epilogue warps add a tile's chunks in registers, rounding to
 // nearest.
+//
+// bf16 and fp16 run as they are (one plane), 4096 of k a chunk: less than 256 x 2^-24 is lost, a sixteenth
+// of fp16's rounding, and calls of up to 4096 of k, with one accumulator a tile, have a kernel without the
+// sums in registers.  It costs nothing (65536 x 1024 x 1024 bf16 gradients 259 us, 278 before; with
+// chunks of 1024, 16384 x 4096 x 4096 takes 354 us instead of 348).  An fp32 operand is the sum of three bf16 planes
+// (3 x 8 significant bits; the differences are exact), and the product is the six plane products
+// that reach 2^-24 of it: a3 b1, a1 b3, a2 b2, a2 b1, a1 b2, a1 b1, smallest first, with a chunk of
+// 64 of k.
 //
 // One CTA per SM walks its tiles: a TMA producer warp, an MMA warp, sixteen epilogue warps.  Two
 // accumulators in TMEM let the epilogue of one tile run beside the next tile's MMAs.
@@ -56,6 +62,7 @@ constexpr uint32_t kTcWait = 1u << 21;   // tries of a wait inside a kernel that
 constexpr int kMaxBn1 = 256, kMaxBn3 = 128;   // rows per tile; three planes' sums are in registers
 constexpr int KB = 64;   // elements of k per stage: a 128-byte row
 constexpr int kMaxStages = 10;
+constexpr int kChunkStages = 64;   // one plane: stages that an accumulator takes at most
 constexpr int kMaxSplit = 8;
 constexpr int kSmemBudget = 217 * 1024;
 constexpr int kSumLanes = 8;
@@ -85,6 +92,7 @@ struct TcOne {
   int64_t rows, chans;      // output rows (N side) and channels (M side)
   int kiters;               // k stages in all
   int per;                  // k stages of one of the CTAs that share a tile's k range
+  int chunk;                // k stages of one accumulator
   int bn;                   // rows per tile
   int tiles_m, tiles_n;     // channel tiles, row tiles
   Divide by_band;           // by the tiles of a band
@@ -258,8 +266,8 @@ __device__ __forceinline__ void emit16(const LinearEpi &e, float (&v)[16], int64
     if (j < n) *p = from_f32<T>(v[j]);
 }
 
-// G CTAs to a tile, P planes per operand.
-template <class T, int G, int P>
+// G CTAs to a tile, P planes per operand; kChunks: a tile's k may take several accumulators.
+template <class T, int G, int P, bool kChunks>
 __global__ void __launch_bounds__(kTcThreads, 1)
     linear_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ TcArgs args, uint32_t *gerr) {
   namespace cg = cooperative_groups;
@@ -273,7 +281,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
   // accumulators: two, or (three planes) two for each team of epilogue warps
-  constexpr int kBuffers = P == 1 ? 2 : 4;
+  constexpr int kTeams = P == 1 ? 1 : 2, kBuffers = 2 * kTeams;
   auto acc_full = [&](int b) { return bar0 + 8u * (2 * kMaxStages + b); };
   auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kMaxStages + 4 + b); };   // rank 0's counts
   const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 8);
@@ -290,7 +298,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     for (int b = 0; b < kBuffers; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), G * (P == 1 ? kEpiWarps : kEpiWarps / 2));
+      mbar_init(acc_empty(b), G * kEpiWarps / kTeams);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -422,7 +430,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t b_adv = g.b_mn ? 2048u >> 4 : 32u >> 4;
         const uint32_t da0 = sdesc_lo(base, g.a_mn ? KB * 128 : 16);
         const uint32_t db0 = sdesc_lo(base + P * a_plane, g.b_mn ? KB * 128 : 16);
-        const int k_hi = at_tile.k_hi, chunk = P == 1 ? g.per : 1;   // stages per accumulator
+        const int k_hi = at_tile.k_hi;
         const int team = P == 1 ? 0 : turn++ & 1;
         int unit = team ? units[1] : units[0];
         for (int k = at_tile.k_lo; k < k_hi && ok; ++unit) {
@@ -433,7 +441,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           tc_fence_after();
           const uint32_t d = uniform(tmem + b * acc_cols);
-          const int k_end = min(k + chunk, k_hi);
+          const int k_end = kChunks ? min(k + g.chunk, k_hi) : k_hi;
           uint32_t accumulate = 0;
           for (; k < k_end; ++k) {
             if (!mbar_wait(full(s), phase, abort_flag, gerr, ERR_WAIT_FULL, kTcWait)) {
@@ -476,7 +484,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else {
     // ---------------- epilogue warps: lanes 32 (warp % 4) .. + 31, every fourth block of 16 columns
-    const int part_of = warp - kFirstEpi, quad = warp & 3, team = part_of >> 3;
+    const int part_of = warp - kFirstEpi, quad = warp & 3, team = P == 1 ? 0 : part_of >> 3;
     const uint32_t tl = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     if (args.sums.parts > 0 && warp < kFirstEpi + kSumLanes) {   // column sums, 32 columns at a time, while the first tile's products run
       float *red = reinterpret_cast<float *>(gbase + kSmemBudget + 512);
@@ -505,7 +513,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int64_t row0 = static_cast<int64_t>(at_tile.tn) * g.bn;
       const float bias = g.e.bias && chan < g.chans ? to_f32(static_cast<const T *>(g.e.bias)[chan]) : 0.0f;
       float *part = reinterpret_cast<float *>(gbase);   // split: [bn][128] of this CTA's part
-      if constexpr (P == 1) {
+      if constexpr (!kChunks) {
         const int b = unit & 1;
         if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC, kTcWait)) break;
         tc_fence_after();
@@ -525,17 +533,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane == 0) arrive<G>(G == 1 ? acc_empty(b) : in_rank0(acc_empty(b)));
         ++unit;
       } else {
-        // Two teams of eight warps take turns at the tiles: one adds up the chunks of a tile while the
-        // other still stores the one before (19434 x 192 x 768 spent 4700 of a tile's 7900 clocks on
-        // its stores with one team).
-        if (turn++ % 2 != team) continue;
-        const int half = (part_of & 7) >> 2;
-        float acc[kMaxBn3 / 32][16];
+        // Three planes: two teams of eight warps take turns at the tiles, one adds up the chunks of a
+        // tile while the other still stores the one before (19434 x 192 x 768 spent 4700 of a tile's
+        // 7900 clocks on its stores with one team).
+        if (kTeams == 2 && turn++ % 2 != team) continue;
+        // a warp's columns: blocks of 16, every kGroups-th
+        constexpr int kGroups = kEpiWarps / kTeams / 4, kBlocks = (P == 1 ? kMaxBn1 : kMaxBn3) / (16 * kGroups);
+        const int c0 = (part_of / 4 % kGroups) * 16;
+        float acc[kBlocks][16];
 #pragma unroll
-        for (int i = 0; i < kMaxBn3 / 32; ++i)
+        for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-        for (int k = at_tile.k_lo; k < at_tile.k_hi && ok; ++k, ++unit) {
+          for (int j = 0; j < 16; ++j) acc[i][j] = -0.0f;   // (what is added to it stays as it is, -0 too)
+        for (int k = at_tile.k_lo; k < at_tile.k_hi && ok; k += g.chunk, ++unit) {
           const int b = 2 * team + (unit & 1);
           if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC, kTcWait)) {
             ok = false;
@@ -543,10 +553,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < kMaxBn3 / 32; ++i) {
-            if (half * 16 + i * 32 < g.bn) {
+          for (int i = 0; i < kBlocks; ++i) {
+            if (c0 + i * 16 * kGroups < g.bn) {
               float v[16];
-              tmem_ld16(tl + b * acc_cols + half * 16 + i * 32, v);
+              tmem_ld16(tl + b * acc_cols + c0 + i * 16 * kGroups, v);
 #pragma unroll
               for (int j = 0; j < 16; ++j) acc[i][j] += v[j];
             }
@@ -560,19 +570,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           // the stages still hold operands of the last chunk until its MMAs are done, which the
           // last accumulator's arrival says
 #pragma unroll
-          for (int i = 0; i < kMaxBn3 / 32; ++i)
-            if (half * 16 + i * 32 < g.bn)
+          for (int i = 0; i < kBlocks; ++i) {
+            const int c = c0 + i * 16 * kGroups;
+            if (c < g.bn)
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                part[(half * 16 + i * 32 + j) * kM + quad * 32 + lane] = acc[i][j];
+              for (int j = 0; j < 16; ++j) part[(c + j) * kM + quad * 32 + lane] = acc[i][j];
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < kMaxBn3 / 32; ++i) {
-            const int c = half * 16 + i * 32;
+          for (int i = 0; i < kBlocks; ++i) {
+            const int c = c0 + i * 16 * kGroups;
             const int n = static_cast<int>(min(static_cast<int64_t>(16), g.rows - row0 - c));
-            if (c < g.bn && chan < g.chans && n > 0) {
-              emit16<T>(g.e, acc[i], chan, row0 + c, n, bias);
-            }
+            if (c < g.bn && chan < g.chans && n > 0) emit16<T>(g.e, acc[i], chan, row0 + c, n, bias);
           }
         }
       }
@@ -792,6 +801,15 @@ Shape pick_shape(const pt_b200_ops *h, int64_t rows, int64_t chans, int kiters, 
 }
 
 template <class T, int P>
+auto *tc_kernel(int group, bool chunks) {
+  if constexpr (P == 3)
+    return group == 1 ? linear_tc_kernel<T, 1, P, true> : linear_tc_kernel<T, 2, P, true>;
+  else
+    return chunks ? (group == 1 ? linear_tc_kernel<T, 1, P, true> : linear_tc_kernel<T, 2, P, true>)
+                  : (group == 1 ? linear_tc_kernel<T, 1, P, false> : linear_tc_kernel<T, 2, P, false>);
+}
+
+template <class T, int P>
 int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes, int count, const ColumnSums &sums,
            bool early, bool beside, int most, cudaStream_t st) {
   constexpr bool kHalf = std::is_same_v<T, __half>;
@@ -802,6 +820,7 @@ int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes,
   a.beside = beside;
   a.split = shapes[0].split;
   a.acc_cols = 16;
+  bool chunks = P == 3;
   for (int i = 0; i < count; ++i) {
     const TcProduct &p = products[i];
     TcOne &g = a.p[i];
@@ -813,6 +832,8 @@ int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes,
     g.kiters = k_stages(p.k);
     g.bn = shapes[i].bn;
     g.per = (g.kiters + a.split - 1) / a.split;
+    g.chunk = P == 1 ? kChunkStages : 1;
+    chunks = chunks || g.per > g.chunk;
     g.tiles_m = static_cast<int>((p.chans + G * kM - 1) / (G * kM));
     const int64_t tiles_n = (p.rows + g.bn - 1) / g.bn;
     PTB_REQUIRE(tiles_n * g.tiles_m < (int64_t(1) << 29) && tiles_n < (int64_t(1) << 26),
@@ -833,7 +854,7 @@ int launch(const pt_b200_ops *h, const TcProduct *products, const Shape *shapes,
   }
   if (count == 1) maps.a[1] = maps.a[0], maps.b[1] = maps.b[0];
   a.stages = std::min<int>(kMaxStages, kSmemBudget / a.stage_bytes);
-  auto kernel = G == 1 ? linear_tc_kernel<T, 1, P> : linear_tc_kernel<T, 2, P>;
+  auto *kernel = tc_kernel<T, P>(G, chunks);
   const int group = G * a.split;
   const int all = a.tiles[0] + a.tiles[1];
   const int workers = a.split > 1 ? all : std::min({all, most, group == 1 ? h->clusters[0] : h->clusters[1]});
@@ -909,12 +930,16 @@ namespace ptb {
 
 int tc_setup(pt_b200_ops *h) {
   const void *const kernels[] = {
-      reinterpret_cast<const void *>(linear_tc_kernel<float, 1, 3>),
-      reinterpret_cast<const void *>(linear_tc_kernel<float, 2, 3>),
-      reinterpret_cast<const void *>(linear_tc_kernel<__nv_bfloat16, 1, 1>),
-      reinterpret_cast<const void *>(linear_tc_kernel<__nv_bfloat16, 2, 1>),
-      reinterpret_cast<const void *>(linear_tc_kernel<__half, 1, 1>),
-      reinterpret_cast<const void *>(linear_tc_kernel<__half, 2, 1>)};
+      reinterpret_cast<const void *>(tc_kernel<float, 3>(1, true)),
+      reinterpret_cast<const void *>(tc_kernel<float, 3>(2, true)),
+      reinterpret_cast<const void *>(tc_kernel<__nv_bfloat16, 1>(1, false)),
+      reinterpret_cast<const void *>(tc_kernel<__nv_bfloat16, 1>(2, false)),
+      reinterpret_cast<const void *>(tc_kernel<__nv_bfloat16, 1>(1, true)),
+      reinterpret_cast<const void *>(tc_kernel<__nv_bfloat16, 1>(2, true)),
+      reinterpret_cast<const void *>(tc_kernel<__half, 1>(1, false)),
+      reinterpret_cast<const void *>(tc_kernel<__half, 1>(2, false)),
+      reinterpret_cast<const void *>(tc_kernel<__half, 1>(1, true)),
+      reinterpret_cast<const void *>(tc_kernel<__half, 1>(2, true))};
   for (const void *k : kernels)
     PTB_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
   for (int log = 0; log < 4; ++log) {
