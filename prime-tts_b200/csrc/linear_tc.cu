@@ -20,13 +20,18 @@
 // accumulator takes a chunk of k, and the epilogue warps add a tile's chunks in registers, rounding to
 // nearest.
 //
-// bf16 and fp16 run as they are (one plane), 4096 of k a chunk: less than 256 x 2^-24 is lost, a sixteenth
+// bf16 and fp16 run as they are (one plane), 4096 of k a chunk: less than 256 x 2^-24 is lost, a thirtieth
 // of fp16's rounding, and calls of up to 4096 of k, with one accumulator a tile, have a kernel without the
 // sums in registers.  It costs nothing (65536 x 1024 x 1024 bf16 gradients 259 us, 278 before; with
-// chunks of 1024, 16384 x 4096 x 4096 takes 354 us instead of 348).  An fp32 operand is the sum of three bf16 planes
-// (3 x 8 significant bits; the differences are exact), and the product is the six plane products
-// that reach 2^-24 of it: a3 b1, a1 b3, a2 b2, a2 b1, a1 b2, a1 b1, smallest first, with a chunk of
-// 64 of k.
+// chunks of 1024, 16384 x 4096 x 4096 takes 354 us instead of 348).
+//
+// An fp32 operand is the sum of three bf16 planes (3 x 8 significant bits; the differences are exact),
+// and the product is the six plane products that reach 2^-24 of it: a3 b1, a1 b3, a2 b2, a2 b1, a1 b2,
+// a1 b1, smallest first, with a chunk of 64 of k.  The second plane is kept 2^7 and the third 2^14 times
+// as large, because bf16 has fp32's exponents: unscaled, operands under 1e-33 lost their low planes (1e-36
+// to an error of 2.7e-5).  The accumulator is taken times 2^-7 where the products go from one pair of
+// scales to the next, which the MMA does on the way and in the same time (19434 x 192 x 768 54.2 us with
+// and without).
 //
 // One CTA per SM walks its tiles: a TMA producer warp, an MMA warp, sixteen epilogue warps.  Two
 // accumulators in TMEM let the epilogue of one tile run beside the next tile's MMAs.
@@ -121,20 +126,28 @@ struct TcMaps {
 
 // ---- the same steps for one CTA (G = 1) and for a pair (G = 2, issued by its rank 0)
 // Descriptors come as their low words (the address moves, 16 bytes a step) and the constant high
-// word; FIRST starts the accumulator where `keep` is 0, any other MMA adds to it.
-template <int G, bool FIRST>
+// word.  kFirst starts the accumulator where `keep` is 0, kShift adds to it after taking it times
+// 2^-kPlaneShift, any other MMA adds to it.
+enum class Acc { kFirst, kShift, kAdd };
+template <int G, Acc ACC>
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
                                         uint32_t keep) {
-#define PTB_MMA(group, pred)                                                                              \
+#define PTB_MMA(group, pred, shift)                                                                       \
   asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"                                               \
                "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t" pred                                   \
-               "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),        \
-               "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(keep)                                       \
+               "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %4, p" shift ";\n\t}" ::"r"(d_tmem), \
+               "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(keep), "n"(kPlaneShift)                     \
                : "memory")
-  if constexpr (G == 1 && FIRST) PTB_MMA("1", "setp.ne.b32 p, %5, 0;\n\t");
-  if constexpr (G == 1 && !FIRST) PTB_MMA("1", "setp.ne.b32 p, 1, 0;\n\t");
-  if constexpr (G == 2 && FIRST) PTB_MMA("2", "setp.ne.b32 p, %5, 0;\n\t");
-  if constexpr (G == 2 && !FIRST) PTB_MMA("2", "setp.ne.b32 p, 1, 0;\n\t");
+#define PTB_KEEP "setp.ne.b32 p, %5, 0;\n\t"
+#define PTB_ALWAYS "setp.ne.b32 p, 1, 0;\n\t"
+  if constexpr (G == 1 && ACC == Acc::kFirst) PTB_MMA("1", PTB_KEEP, "");
+  if constexpr (G == 1 && ACC == Acc::kShift) PTB_MMA("1", PTB_ALWAYS, ", %6");
+  if constexpr (G == 1 && ACC == Acc::kAdd) PTB_MMA("1", PTB_ALWAYS, "");
+  if constexpr (G == 2 && ACC == Acc::kFirst) PTB_MMA("2", PTB_KEEP, "");
+  if constexpr (G == 2 && ACC == Acc::kShift) PTB_MMA("2", PTB_ALWAYS, ", %6");
+  if constexpr (G == 2 && ACC == Acc::kAdd) PTB_MMA("2", PTB_ALWAYS, "");
+#undef PTB_KEEP
+#undef PTB_ALWAYS
 #undef PTB_MMA
 }
 // Arrives on the barrier at this offset, of both CTAs of a pair, once the MMAs so far are done.
@@ -457,12 +470,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const uint32_t da = da0 + here + (P == 1 ? 0 : kPa[q]) * (a_plane >> 4);
                 const uint32_t db = db0 + here + (P == 1 ? 0 : kPb[q]) * (b_plane >> 4);
                 if (q == 0)
-                  mma_f16<G, true>(d, da, db, kDescHi, g.idesc, first_of);
+                  mma_f16<G, Acc::kFirst>(d, da, db, kDescHi, g.idesc, first_of);
+                else if (kPa[q] + kPb[q] < kPa[q - 1] + kPb[q - 1])   // the next planes: what is there is shifted
+                  mma_f16<G, Acc::kShift>(d, da, db, kDescHi, g.idesc, 1);
                 else
-                  mma_f16<G, false>(d, da, db, kDescHi, g.idesc, 1);
+                  mma_f16<G, Acc::kAdd>(d, da, db, kDescHi, g.idesc, 1);
 #pragma unroll
                 for (int i = 1; i < KB / 16; ++i)
-                  mma_f16<G, false>(d, da + i * a_adv, db + i * b_adv, kDescHi, g.idesc, 1);
+                  mma_f16<G, Acc::kAdd>(d, da + i * a_adv, db + i * b_adv, kDescHi, g.idesc, 1);
               }
               commit<G>(free_bar);
             }

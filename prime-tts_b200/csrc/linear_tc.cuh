@@ -20,9 +20,13 @@ struct TcProduct {
   LinearEpi e;
 };
 
-// fp32 as the sum of three bf16 values.  One that is not finite lies in the first alone; one that
-// would round up to infinity is truncated there instead.
+// fp32 as three bf16 values, x = o0 + 2^-7 o1 + 2^-14 o2: each is under 2^-8 of the one before (2^-7
+// where that was truncated), so the scaled ones stay below x and reach bf16's smallest numbers no sooner
+// than x itself.  A value that is not finite lies in the first alone; one that would round up to infinity
+// is truncated there instead.
+constexpr int kPlaneShift = 7;
 __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&o)[3]) {
+  constexpr float kUp = 1 << kPlaneShift;
   o[0] = __float2bfloat16_rn(x);
   if (!(fabsf(x) <= 3.38953139e38f)) {   // beyond the largest finite bf16, or NaN
     if (!isfinite(x)) {
@@ -31,9 +35,9 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&o)[3]) {
     }
     o[0] = __float2bfloat16_rz(x);
   }
-  const float r1 = x - __bfloat162float(o[0]);
+  const float r1 = (x - __bfloat162float(o[0])) * kUp;
   o[1] = __float2bfloat16_rn(r1);
-  o[2] = __float2bfloat16_rn(r1 - __bfloat162float(o[1]));
+  o[2] = __float2bfloat16_rn((r1 - __bfloat162float(o[1])) * kUp);
 }
 
 // One pass over a matrix that makes an operand of it: dst receives src * act'(pre) (src itself

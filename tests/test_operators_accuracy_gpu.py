@@ -56,3 +56,75 @@ def test_long_sums_of_one_sign_are_not_biased(ops, dtype, which):
         want = a.double().T @ b.double()
     off = ((got.double() - want) / want).mean().abs().item()
     assert off <= 256 * 2.0 ** -24 + 6 * U[dtype] / n, off
+
+
+def _norm_error(got, want):
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+def _products(ops, x, w, dy):
+    """The three products of a layer with their exact values and their lengths."""
+    dx, dw, _ = ops.linear_backward(dy, x, w)
+    xd, wd, dd = x.double(), w.double(), dy.double()
+    return [("y", ops.linear(x, w), xd @ wd.T, x.shape[1]), ("dx", dx, dd @ wd, w.shape[0]),
+            ("dw", dw, dd.T @ xd, x.shape[0])]
+
+
+SHAPES = [(600, 768, 192), (300, 2056, 136), (257, 193, 515), (40, 9000, 136), (3616, 192, 768), (4, 4096, 1024),
+          (9500, 130, 25)]
+
+
+def _bound(k):
+    """Relative 2-norm error of an fp32 product of k random terms: a chunk of 64 ends in four truncating
+    additions (under 2^-23 each of what is there, half of that on average), k / 64 chunks are added with
+    rounding to nearest, whose errors add up as a random walk does, and the terms' own errors (the products
+    left out, the third planes' rounding) are under 2^-24 and as random as the terms."""
+    return (4 + math.sqrt(k / 64)) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("rows,n_in,n_out", SHAPES)
+def test_f32_products_hold_all_their_bits(ops, rows, n_in, n_out):
+    g = _gen(rows)
+    x, w, dy = _randn(g, rows, n_in), _randn(g, n_out, n_in), _randn(g, rows, n_out)
+    for name, got, want, k in _products(ops, x, w, dy):
+        assert _norm_error(got, want) <= _bound(k), name
+
+
+# x dy and w scales that leave every product a normal number; 1.2e-38 is the smallest normal number, so some of
+# the values themselves are denormal there
+@pytest.mark.parametrize("sx,sw", [(1e-30, 1.0), (1e-34, 1.0), (1e-36, 10.0), (2e-38, 1000.0), (1e-18, 1e-17),
+                                   (1.0, 1e-36), (1e30, 1e-34)])
+@pytest.mark.parametrize("rows", [4, 600])
+def test_f32_products_of_small_operands(ops, rows, sx, sw):
+    g = _gen(7)
+    x, w, dy = sx * _randn(g, rows, 192), sw * _randn(g, 256, 192), _randn(g, rows, 256)
+    for name, got, want, k in _products(ops, x, w, dy):
+        assert _norm_error(got, want) <= _bound(k), name
+    for name, got, want, k in _products(ops, _randn(g, rows, 192), w, sx * dy):
+        assert _norm_error(got, want) <= _bound(k), name
+
+
+def test_bf16_products_of_small_operands(ops):
+    """Rounded once, so under u of every output; normal numbers throughout."""
+    g = _gen(8)
+    for rows in (4, 600):
+        x, w = (1e-30 * _randn(g, rows, 192)).bfloat16(), _randn(g, 256, 192).bfloat16()
+        dy = _randn(g, rows, 256).bfloat16()
+        for name, got, want, k in _products(ops, x, w, dy):
+            assert _norm_error(got, want) <= U[torch.bfloat16], name
+
+
+# x0 w0 + x1 w1: what is left of two terms that all but cancel lies in the product of two of the three parts
+# (8 bits each) that an operand has; every step is exact
+@pytest.mark.parametrize("x0,w0,x1,w1,want", [
+    (1 + 2.0 ** -20, 1, -1, 1, 2.0 ** -20), (1, 1 + 2.0 ** -20, -1, 1, 2.0 ** -20),
+    (1 + 2.0 ** -10, 1, -1, 1, 2.0 ** -10), (1, 1 + 2.0 ** -10, -1, 1, 2.0 ** -10),
+    (1 + 2.0 ** -10, 1 + 2.0 ** -10, -1, 1 + 2.0 ** -9, 2.0 ** -20), (1, 1, 1, -0.5, 0.5)])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -118, 2.0 ** 100])
+def test_f32_terms_that_cancel(ops, x0, w0, x1, w1, want, scale):
+    for rows, at in ((4, 1), (300, 1), (300, 15), (300, 63), (300, 150)):   # one MMA, one chunk, two chunks
+        x, w = torch.zeros(rows, 192, device="cuda"), torch.zeros(200, 192, device="cuda")
+        x[:, 0], x[:, at], w[:, 0], w[:, at] = x0 * scale, x1 * scale, w0, w1
+        assert (ops.linear(x, w) == want * scale).all()
+        dx, _, _ = ops.linear_backward(x, torch.zeros(rows, 200, device="cuda"), w.T.contiguous())
+        assert (dx == want * scale).all()
