@@ -128,3 +128,32 @@ def test_f32_terms_that_cancel(ops, x0, w0, x1, w1, want, scale):
         assert (ops.linear(x, w) == want * scale).all()
         dx, _, _ = ops.linear_backward(x, torch.zeros(rows, 200, device="cuda"), w.T.contiguous())
         assert (dx == want * scale).all()
+
+
+def test_gelu_value_and_slope(ops):
+    """E is fp32's unit roundoff.  h = Phi(-|p|) comes from a fit good to 1.1e-8 and to 1.1e-6 of h, an exponential
+    whose argument carries three roundings (1.5 p^2 E of h), and some sixteen E for the exponential, the
+    reciprocal and the arithmetic; 1 - h rounds once more.  Below 1e-37 the exponential ends."""
+    e = 2.0 ** -24
+    p = torch.linspace(-14, 14, 700001, device="cuda", dtype=torch.float64).float()
+    p = torch.cat([p, torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e30, -1e30, 20.0, -20.0, 100.0, -100.0], device="cuda")])
+    p = torch.cat([p, 3 * _randn(_gen(5), 300000)])[:, None]
+    pd = p.double()
+    h, phi = 0.5 * torch.erfc(pd.abs() * math.sqrt(0.5)), torch.exp(-0.5 * pd * pd) / math.sqrt(2 * math.pi)
+    cdf = torch.where(pd < 0, h, 1 - h)
+    e_exp = (1.5 * pd * pd + 16) * e
+    e_cdf = torch.minimum(torch.full_like(h, 1.1e-8), 1.1e-6 * h) + h * e_exp + torch.where(pd < 0, 0.0, e / 2) + 1e-37
+    one = torch.ones(1, 1, device="cuda")
+    y, pre = ops.linear(p, one, act="gelu", save_pre=True)
+    assert torch.equal(pre, p)
+    value = pd * cdf
+    over = ((y.double() - value).abs() - pd.abs() * e_cdf - e * value.abs()).max().item()
+    assert over <= 0, over
+    slope = cdf + pd * phi
+    dx, _, _ = ops.linear_backward(torch.ones_like(p), p, one, pre=p, act="gelu")
+    e_slope = e_cdf + (pd * phi).abs() * e_exp + pd.abs() * 1e-37 + 2 * e * (cdf + (pd * phi).abs())
+    over = ((dx.double() - slope).abs() - e_slope).max().item()
+    assert over <= 0, over
+    n = _randn(_gen(6), 1 << 20, 1)
+    off = (ops.linear(n, one, act="gelu").double() - torch.nn.functional.gelu(n.double())).square().mean().sqrt().item()
+    assert off <= 3e-8, off     # half a rounding of values of about one
