@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(kBlock) norm_cols_wide_kernel(const NormArgs a
 }
 
 // [parts][n] -> out[n] (and out2 from out_n on): 32 columns x LANES per block; a lane adds every
-// LANES-th partial in order, then the lanes are added in order.
+// LANES-th partial (lane_sum), then the lanes are added in order.
 template <class T, int LANES>
 __global__ void __launch_bounds__(32 * LANES)
     reduce_columns_kernel(const float *__restrict__ part, int parts, int64_t n, T *__restrict__ out,
@@ -549,9 +549,7 @@ __global__ void __launch_bounds__(32 * LANES)
   const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + (threadIdx.x & 31);
   const int lane = threadIdx.x >> 5;
   float v = 0.0f;
-  if (c < n)
-#pragma unroll 8
-    for (int p = lane; p < parts; p += LANES) v += part[p * n + c];
+  if (c < n) v = lane_sum(part + c, lane, parts, LANES, n);
   s[lane][threadIdx.x & 31] = v;
   __syncthreads();
   if (threadIdx.x < 32 && c < n) {

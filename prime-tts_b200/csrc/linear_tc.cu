@@ -506,9 +506,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int row = warp - kFirstEpi;
       for (int64_t c0 = blockIdx.x * 32; c0 < args.sums.n; c0 += gridDim.x * 32) {
         float v = 0.0f;
-        if (c0 + lane < args.sums.n)
-#pragma unroll 4
-          for (int p = row; p < args.sums.parts; p += kSumLanes) v += args.sums.part[p * args.sums.n + c0 + lane];
+        if (c0 + lane < args.sums.n) v = lane_sum(args.sums.part + c0 + lane, row, args.sums.parts, kSumLanes, args.sums.n);
         red[row * 33 + lane] = v;
         asm volatile("bar.sync 1, %0;" ::"n"(kSumLanes * 32) : "memory");
         if (row == 0 && c0 + lane < args.sums.n) {

@@ -157,3 +157,15 @@ def test_gelu_value_and_slope(ops):
     n = _randn(_gen(6), 1 << 20, 1)
     off = (ops.linear(n, one, act="gelu").double() - torch.nn.functional.gelu(n.double())).square().mean().sqrt().item()
     assert off <= 3e-8, off     # half a rounding of values of about one
+
+
+@pytest.mark.parametrize("which", ["alone", "whole"])
+def test_f32_bias_gradient(ops, which):
+    """A chain of n fp32 additions of random terms of equal size has a relative error of E sqrt((n + 1) / 6).  The
+    sum over 3616 rows of 192 columns is one of eight rows in a block, of 452 blocks' sums over eight lanes and
+    four turns (15), of those four in pairs (two levels), and of the eight lanes."""
+    g = _gen(9)
+    x, w, dy = _randn(g, 3616, 768), _randn(g, 192, 768), _randn(g, 3616, 192)
+    alone = dict(need_dx=False, need_dw=False) if which == "alone" else {}
+    db = ops.linear_backward(dy, x, w, **alone)[2]
+    assert _norm_error(db, dy.double().sum(0)) <= 2.0 ** -24 * math.sqrt((9 + 16 + 3 + 9) / 6)
