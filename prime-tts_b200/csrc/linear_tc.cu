@@ -48,6 +48,7 @@
 #include <algorithm>
 #include <climits>
 
+#include "drain.h"
 #include "linear_tc.cuh"
 #include "ptx.cuh"
 
@@ -279,6 +280,21 @@ __device__ __forceinline__ void emit16(const LinearEpi &e, float (&v)[16], int64
     if (j < n) *p = from_f32<T>(v[j]);
 }
 
+// Copies in flight must land before shared memory is given up, whichever producer issued them.  (Not inlined:
+// nothing is live where it is called, and no call that ends as it should comes here.)
+__device__ __noinline__ void drain_copies(uint32_t full, int stages, int a, int b, int lane, uint32_t *gerr) {
+  const Drain d = drain_of(a, b, stages);
+  for (int i = d.begin; i < d.end; ++i) {
+    const uint32_t bar = full + 8u * (i % stages);
+    if (i >= d.matched && lane == 0) mbar_arrive(bar);
+    __syncwarp();
+    uint32_t it = 0;
+    while (!mbar_try_wait(bar, fill_parity(i, stages)) && ++it < kTcWait) {
+    }
+    if (it >= kTcWait && lane == 0) atomicOr(gerr, ERR_WAIT_DRAIN);
+  }
+}
+
 // G CTAs to a tile, P planes per operand; kChunks: a tile's k may take several accumulators.
 template <class T, int G, int P, bool kChunks>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -300,6 +316,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const uint32_t drain = bar0 + 8u * (2 * kMaxStages + 8);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gbase + kSmemBudget + 8 * (2 * kMaxStages + 9));
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  int *issued_of = reinterpret_cast<int *>(tmem_slot + 2);   // stages that the producers have copied, B's and A's
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t tmem_cols = kBuffers * acc_cols;
@@ -421,17 +438,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (++s == args.stages) s = 0, phase ^= 1u, a0 -= args.stages * stage_bytes;
       }
     }
-    if (!ok && pair_rank == 0 && is_a) {   // copies in flight must land before shared memory is given up
-      const int flying = min(issued, args.stages);
-      for (int i = 0; i < flying; ++i) {
-        if (s == 0) s = args.stages, phase ^= 1u;
-        --s;
-        uint32_t it = 0;
-        while (!mbar_try_wait(full(s), phase) && ++it < kTcWait) {
-        }
-        if (it >= kTcWait && one) atomicOr(gerr, ERR_WAIT_DRAIN);
-      }
-    }
+    if (lane == 0) issued_of[is_a] = issued;
   } else if (warp == 1) {
     if (pair_rank == 0) {
       // ---------------- MMA issuer
@@ -634,6 +641,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (warp == 0 && pair_rank == 0 && *abort_flag) {
+    // a role gave up (a pair's copies count on rank 0's barriers; rank 1 stops only after a wait of its own)
+    drain_copies(full(0), args.stages, issued_of[1], issued_of[0], lane, gerr);
+  }
   if constexpr (G == 2) cg::this_cluster().sync();   // nor while the pair's MMAs or arrivals reach it
   if (warp == 1) {
     tc_fence_after();
