@@ -280,8 +280,8 @@ __device__ __forceinline__ void emit16(const LinearEpi &e, float (&v)[16], int64
     if (j < n) *p = from_f32<T>(v[j]);
 }
 
-// Copies in flight must land before shared memory is given up, whichever producer issued them.  (Not inlined:
-// nothing is live where it is called, and no call that ends as it should comes here.)
+// Waits for the copies that two producers have issued.  (Not inlined: nothing is live where it is called, and
+// no call that ends as it should comes here.)
 __device__ __noinline__ void drain_copies(uint32_t full, int stages, int a, int b, int lane, uint32_t *gerr) {
   const Drain d = drain_of(a, b, stages);
   for (int i = d.begin; i < d.end; ++i) {
@@ -439,6 +439,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     }
     if (lane == 0) issued_of[is_a] = issued;
+    if (pair_rank == 0) asm volatile("bar.arrive 2, 96;" ::: "memory");   // both producers are through: for the MMA warp
   } else if (warp == 1) {
     if (pair_rank == 0) {
       // ---------------- MMA issuer
@@ -500,7 +501,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         (team ? units[1] : units[0]) = unit;
       }
-      if (!ok) {   // MMAs already issued must finish before TMEM is released
+      asm volatile("bar.sync 2, 96;" ::: "memory");
+      if (!ok) {
+        // copies in flight must land before shared memory is given up, whichever producer issued them (a
+        // pair's count on rank 0's barriers; rank 1 stops only after a wait of its own), and MMAs already
+        // issued must finish before TMEM is
+        drain_copies(full(0), args.stages, issued_of[1], issued_of[0], lane, gerr);
         if (one) commit<G>(drain);
         uint32_t it = 0;
         while (!mbar_try_wait(drain, 0) && ++it < kTcWait) {
@@ -641,10 +647,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0 && pair_rank == 0 && *abort_flag) {
-    // a role gave up (a pair's copies count on rank 0's barriers; rank 1 stops only after a wait of its own)
-    drain_copies(full(0), args.stages, issued_of[1], issued_of[0], lane, gerr);
-  }
   if constexpr (G == 2) cg::this_cluster().sync();   // nor while the pair's MMAs or arrivals reach it
   if (warp == 1) {
     tc_fence_after();
