@@ -425,19 +425,23 @@ PT_B200_API int pt_b200_conv_noalloc(int device, void *stream, const float *x, i
  * Every matrix is row-major with a row stride in elements (at least its column count); rows need
  * no alignment beyond their element's.  All tensors of a call have one element type.  Sums,
  * statistics and activations are computed in fp32 and rounded once, to nearest, when stored; an
- * fp32 call keeps 32-bit accuracy in its products (an infinite fp32 input makes the outputs that
- * depend on it NaN or infinite).  Calls are asynchronous on `stream` (NULL: the default stream)
- * and allocate nothing: workspace (256-byte aligned) comes from the caller, sized by the *_work
- * function for the same arguments, and is free for reuse once the call's work on the stream is
- * done.  The status covers argument and launch errors; pt_b200_ops_sync waits for the stream and
- * reports device errors.  Results do not depend on timing: the same call gives the same bits.
+ * fp32 call keeps 32-bit accuracy in its products, down to fp32's smallest normal numbers.  An
+ * infinite fp32 input of a linear layer or its gradient makes the outputs that depend on it
+ * infinite or NaN: the tensor-core kernels, which calls of more than a few rows take, give NaN
+ * also where the exact value is infinite (and so NaN instead of 0 behind relu).  Calls are
+ * asynchronous on `stream` (NULL: the default stream) and allocate nothing: workspace (256-byte
+ * aligned) comes from the caller, sized by the *_work function for the same arguments, and is free
+ * for reuse once the call's work on the stream is done.  The status covers argument and launch
+ * errors, a pointer that is not aligned to its element among them; pt_b200_ops_sync waits for the
+ * stream and reports device errors, once, of any of the handle's calls so far.  Results do not
+ * depend on timing: the same call gives the same bits.
  * A handle may be used by several threads and streams at once. */
 enum { PT_B200_F32 = 0, PT_B200_BF16 = 1, PT_B200_F16 = 2 };
 /* Activations; 1 and 2 are the conv entry points' epilogue codes. */
 enum {
   PT_B200_ACT_NONE = 0,
-  PT_B200_ACT_LEAKY = 1, /* p < 0 ? slope * p : p */
-  PT_B200_ACT_RELU = 2,  /* p < 0 ? 0 : p */
+  PT_B200_ACT_LEAKY = 1, /* p < 0 ? slope * p : p; its slope at 0 is 1 */
+  PT_B200_ACT_RELU = 2,  /* p < 0 ? 0 : p; its slope at 0 is 0 */
   PT_B200_ACT_GELU = 5,  /* p * Phi(p), Phi the normal distribution function */
   PT_B200_ACT_SILU = 6   /* p / (1 + exp(-p)) */
 };

@@ -280,10 +280,19 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
          n_out < (int64_t(1) << 30);
 }
 
-// The kernel that a call takes: by the microseconds that each would take.  Its own follow
+// Whether x and w can be read 16 bytes at a time.
+bool copies_whole(const pt_b200_linear_args *p) {
+  const int v = 16 / dtype_bytes(p->dtype);
+  auto aligned = [&](const void *q, int64_t rows, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows == 1 || ld % v == 0);
+  };
+  return p->in % v == 0 && aligned(p->x, p->rows, p->ldx) && aligned(p->w, p->out, p->ldw);
+}
+
+// The kernel that a call takes: by the microseconds that each would take.  The few-rows kernel's follow
 // from its warps' tasks (two channels x eight rows), each a start and k; the tensor cores' from a start,
-// the first stages of k, the weights and x (in its planes, against a tile of 128 channels).  Fits to measurements (the tensor cores' in brackets, rows x
-// in x out):
+// the first stages of k, the weights and x (in its planes, against a tile of 128 channels).  Fits to
+// measurements (the tensor cores' in brackets, rows x in x out):
 //   bf16  4 x 4096 x 1024 4.5 (6.8), 8 x 1024 x 1024 3.9 (5.9), 2 x 4096 x 4096 7.4 (8.8), 4 x 4096 x
 //         4096 10.5 (8.8), 64 x 192 x 768 5.7 (4.9), 1000 x 64 x 64 6.2 (4.5)
 //   not aligned, so that the tensor cores need copies: 128 x 101 x 201 4.4 (5.9), 500 x 101 x 201 10.1
@@ -294,14 +303,6 @@ bool sizes_ok(int64_t rows, int64_t n_in, int64_t n_out) {
 // The few-rows kernel waits for an x that does not stay in L2.  The narrow one takes a start and, for each
 // 64 rows on an SM, steps of k: 1000 x 4096 x 32 73 us (few rows 15.5), 4000 x 1024 x 16 15 (10.5), 2000 x
 // 192 x 16 5.5 (3.3), 7369 x 2296 x 24 45 (46), 19434 x 192 x 32 13.9 (tensor cores 19.9).
-// Whether x and w can be read 16 bytes at a time.
-bool copies_whole(const pt_b200_linear_args *p) {
-  const int v = 16 / dtype_bytes(p->dtype);
-  auto aligned = [&](const void *q, int64_t rows, int64_t ld) {
-    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && (rows == 1 || ld % v == 0);
-  };
-  return p->in % v == 0 && aligned(p->x, p->rows, p->ldx) && aligned(p->w, p->out, p->ldw);
-}
 enum class Way { kTensor, kFew, kNarrow };
 constexpr int kFewRows = 1 << 18;
 Way way(const pt_b200_ops *h, const pt_b200_linear_args *p) {
