@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int i = 0; i < kBlocks; ++i)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) acc[i][j] = -0.0f;   // (what is added to it stays as it is, -0 too)
+          for (int j = 0; j < 16; ++j) acc[i][j] = P == 1 ? -0.0f : 0.0f;   // (-0 leaves a single chunk's bits as they are)
         for (int k = at_tile.k_lo; k < at_tile.k_hi && ok; k += chunk_of(g), ++unit) {
           const int b = 2 * team + (unit & 1);
           if (!mbar_wait(acc_full(b), (unit >> 1) & 1, abort_flag, gerr, ERR_WAIT_ACC, kTcWait)) {
