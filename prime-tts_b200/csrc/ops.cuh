@@ -102,7 +102,7 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // those of the least largest error on 0 <= p <= 14.5 in the weight h^(1/2) (Lawson's iteration of weighted
 // least squares): 1.0e-8 of h in all, and 1.1e-6 relative out to h = 1e-47, so that gelu's left tail keeps
 // its digits.  (Degree 6 leaves 5.9e-8.  Abramowitz and Stegun's 7.1.26, one term less still, is off by
-// 7.5e-8: gelu of normal arguments had an error of 5.7e-8, and has 2.5e-8 now, an fp32 erf's.)  The
+// 7.5e-8: gelu of normal arguments had an error of 5.7e-8, and has 2.6e-8 now, as an fp32 erf.)  The
 // exponential is also the density's, so value and slope of gelu cost one exponential and one reciprocal.
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
